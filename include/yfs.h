@@ -345,6 +345,34 @@ int yfs_mask_to_boxes_u8(const uint8_t *mask, int64_t N, int H, int W, int CH, c
 int yfs_anchor_assign_f32(const float *wh, int64_t n, const float *anchors, int k, int32_t *assign, float *best_iou,
                           void *stream);
 
+/* ---- operators of the fully connected head (no reference code; the head is yolo_toy_regressor_torch.py:258-266) --------- */
+
+typedef enum { YFS_F32 = 0, YFS_BF16 = 1, YFS_F16 = 2 } yfs_dtype;
+
+/* Layer norm over the last axis: y = (x - mu) / sqrt(v + eps) * w + b with the row's mean mu and biased variance v, all in
+ * fp32 with one rounding at the end.  x [rows, cols] with x_stride elements from row to row (0: one row for all), y [rows,
+ * cols] dense, both `dtype`; w, b [cols] fp32 or NULL (ones / zeros); mean, rstd [rows] fp32 or NULL: what the backward
+ * pass needs. */
+int yfs_layer_norm_fwd(const void *x, int64_t x_stride, const float *w, const float *b, void *y, float *mean, float *rstd,
+                       int64_t rows, int64_t cols, float eps, int dtype, void *stream);
+/* g = dy w; dx = rstd (g - mean(g) - h mean(g h)) with h = (x - mean) rstd; dw = sum over rows of dy h; db = sum over rows
+ * of dy.  dx (dense, `dtype`), dw, db (fp32 [cols]) may each be NULL.  Deterministic: the rows are summed in a fixed order. */
+size_t yfs_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols, int dtype);
+int yfs_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, const float *w, const float *mean,
+                       const float *rstd, void *dx, float *dw, float *db, int64_t rows, int64_t cols, int dtype,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
+/* LeakyReLU(slope) and dropout(p) whose mask is never stored: element e (row-major) is kept iff
+ * (philox4x32_10(key = seed, counter = e / 4)[e % 4] >> 8) * 2^-24 >= p, the rule of yfs_fc_epilogue_fwd_bf16.
+ * fwd: y = keep ? leaky(x) / (1 - p) : 0.  bwd: dx = keep ? dy / (1 - p) * (y > 0 ? 1 : slope) : 0; y is read only when
+ * slope != 1 (1: no activation).  n elements of `dtype`; 0 <= p <= 1, 0 <= slope <= 1.  seed_dev (may be NULL): a seed in
+ * device memory that replaces `seed` and is read when the kernel runs, so that a captured graph draws a new mask at every
+ * replay that changes it.  x == y and dy == dx are allowed. */
+int yfs_dropout_fwd(const void *x, void *y, int64_t n, float p, float slope, uint64_t seed, const int64_t *seed_dev, int dtype,
+                    void *stream);
+int yfs_dropout_bwd(const void *dy, const void *y, void *dx, int64_t n, float p, float slope, uint64_t seed,
+                    const int64_t *seed_dev, int dtype, void *stream);
+
 /* Measurement aid, no reference counterpart: enqueue a register-only bf16 MFMA loop (blocks x 4 waves x iters x
  * 16 MFMAs of 16x16x32) and return the FLOPs it performs in *flop_out; the caller times it.  scratch: >= 4 bytes of
  * device memory (never written in practice).  bench.py prints the resulting rate next to the vendor peak. */

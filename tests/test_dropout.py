@@ -1,0 +1,200 @@
+"""Dropout without a stored mask (yolo_from_scratch_amd.dropout, HipDropout): which elements are kept is compared exactly
+with the oracle (Philox pinned by its known answer in test_fc_epilogue.py), values to one rounding: half a step of the type,
+and 3 steps of 2^-24 for the fp32 products with slope and 1 / (1 - p) (itself rounded once)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import head_ref as hr
+
+DEV = "cuda:0"
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _close(got, ref, dtype):
+    tol = (torch.finfo(dtype).eps / 2 + 4 * 2.0 ** -24) * np.abs(ref) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    assert np.array_equal(got == 0, np.abs(ref) == 0) or dtype == torch.float16
+    bad = ~(np.abs(got - ref) <= tol)
+    assert not bad.any(), f"{bad.sum()} of {bad.size} off"
+
+
+def _check(x, dy, p, seed, slope, seed_arg=None):
+    import yolo_from_scratch_amd as yfs
+    xg = x.detach().requires_grad_()
+    y = yfs.dropout(xg, p, seed if seed_arg is None else seed_arg, slope)
+    dx, = torch.autograd.grad(y, xg, dy)
+    assert y.dtype == x.dtype and y.shape == x.shape and dx.shape == x.shape and y.is_contiguous()
+    _close(_np(y), hr.dropout(_np(x), p, seed, slope), x.dtype)
+    _close(_np(dx), hr.dropout_bwd(_np(dy), _np(y), p, seed, slope), x.dtype)
+    with torch.no_grad():
+        assert torch.equal(yfs.dropout(x, p, seed if seed_arg is None else seed_arg, slope), y)
+    return y, dx
+
+
+def test_refusals():
+    import yolo_from_scratch_amd as y
+    x = torch.zeros(4, 8)
+    for call in (lambda: y.dropout(x, 0.1, 1), lambda: y.dropout(x.double(), 0.1, 1), lambda: y.dropout(x, -0.1, 1),
+                 lambda: y.dropout(x, 1.1, 1), lambda: y.dropout(x, float("nan"), 1), lambda: y.dropout(x, 0.1, 1, -0.5),
+                 lambda: y.dropout(x, 0.1, 1, 1.5), lambda: y.dropout(x, 0.1, 1.0), lambda: y.dropout(x, 0.1, None),
+                 lambda: y.dropout(x, 0.1, torch.zeros(2, dtype=torch.int64)), lambda: y.dropout(x, 0.1, torch.zeros(1)),
+                 lambda: y.HipDropout(1.5), lambda: y.HipDropout(0.5, -1.0)):
+        with pytest.raises(y.YfsError):
+            call()
+    lib, one = y.lib(), 4096
+    assert lib.yfs_dropout_fwd(None, one, 8, 0.1, 1.0, 1, None, 0, None) == -1
+    assert lib.yfs_dropout_fwd(one, one, 0, 0.1, 1.0, 1, None, 0, None) == -1
+    assert lib.yfs_dropout_fwd(one, one, 8, 1.5, 1.0, 1, None, 0, None) == -1
+    assert lib.yfs_dropout_fwd(one, one, 8, 0.5, 2.0, 1, None, 0, None) == -1
+    assert lib.yfs_dropout_fwd(one, one, 8, 0.5, 1.0, 1, None, 7, None) == -2
+    assert lib.yfs_dropout_bwd(one, None, one, 8, 0.5, 0.1, 1, None, 0, None) == -1
+
+
+def test_oracle_backward_against_differences():
+    rng = np.random.default_rng(3)
+    x, dy, v = rng.standard_normal((3, 7, 41))
+    y = hr.dropout(x, 0.3, 77, 0.1)
+    s = 1e-7                                       # no element changes its sign within s
+    diff = (dy * (hr.dropout(x + s * v, 0.3, 77, 0.1) - hr.dropout(x - s * v, 0.3, 77, 0.1))).sum() / (2 * s)
+    np.testing.assert_allclose((hr.dropout_bwd(dy, y, 0.3, 77, 0.1) * v).sum(), diff, rtol=1e-6)
+    assert abs(hr.keep_mask(5, 100000, 0.3).mean() - 0.7) < 0.01
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 7, 8, 9, 15, 17, 255, 2048, 2049, 4099, 100003])
+@pytest.mark.parametrize("p,slope", [(0.2, 0.1), (0.5, 1.0), (0.0, 0.1), (0.0, 1.0), (1.0, 1.0), (1.0, 0.1), (0.999, 0.0)])
+def test_against_oracle(n, dtype, p, slope):
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, generator=g).to(DTYPES[dtype]).to(DEV)
+    dy = torch.randn(n, generator=g).to(DTYPES[dtype]).to(DEV)
+    _check(x, dy, p, 0x9E3779B97F4A7C15 + n, slope)
+
+
+@pytest.mark.gpu
+def test_same_mask_as_the_fused_epilogue():
+    import yolo_from_scratch_amd as yfs
+    from yolo_from_scratch_amd import fc_ops as fo
+    part = torch.randn(1, 48, 1480, device=DEV)
+    for p in (0.2, 0.5):
+        y, keep = fo.fc_epilogue_fwd(part, None, 0.1, p, 987654321)
+        mine = yfs.dropout(part[0], p, 987654321, 0.1)
+        assert torch.equal(mine != 0, keep.bool())
+        assert float((mine - y.float()).abs().max()) <= 2.0 ** -8 * float(mine.abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_views_and_special_values(dtype):
+    """Odd offsets, transposed and expanded tensors follow the row-major order of the view; what is dropped leaves zero even
+    where the input is NaN or infinite; zeros, negative zeros and infinities that are kept."""
+    import yolo_from_scratch_amd as yfs
+    t = DTYPES[dtype]
+    base = torch.randn(50, 61, device=DEV).to(t)
+    for x in (base.flatten()[1:1001], base.t(), base[3:4].expand(6, 61), base[::3, 1::2], base.view(5, 2, 5, 61)):
+        _check(x, torch.randn(x.shape, device=DEV).to(t), 0.3, 4242, 0.1)
+    x = base.clone()
+    x[:, 0], x[:, 1], x[:, 2], x[:, 3], x[:, 4] = float("nan"), float("inf"), -float("inf"), 0.0, -0.0
+    keep = torch.from_numpy(hr.keep_mask(11, x.numel(), 0.5)).view(x.shape).to(DEV)
+    y = yfs.dropout(x, 0.5, 11, 0.1)
+    assert (y[~keep] == 0).all() and torch.isfinite(y[~keep]).all()
+    assert y[:, 0][keep[:, 0]].isnan().all()
+    assert (y[:, 1][keep[:, 1]] == float("inf")).all() and (y[:, 2][keep[:, 2]] == -float("inf")).all()
+    e = torch.empty(0, 4, device=DEV, dtype=t, requires_grad=True)
+    ye = yfs.dropout(e, 0.5, 1)
+    assert ye.shape == (0, 4) and torch.autograd.grad(ye.sum(), e)[0].shape == (0, 4)
+
+
+@pytest.mark.gpu
+def test_counter_is_the_element_index_past_32_bits():
+    """An fp16 tensor of 2^32 + 4096 elements (8 GiB): the last elements use counters of their own."""
+    import yolo_from_scratch_amd as yfs
+    from oracle.fc_ref import philox4x32_10
+    n = (1 << 32) + 4096
+    x = torch.ones(n, device=DEV, dtype=torch.float16)
+    y = yfs.dropout(x, 0.5, 31337)
+    tail = 8192
+    r = philox4x32_10(31337, np.arange((n - tail) // 4, n // 4, dtype=np.uint64)).reshape(-1)
+    want = (r >> np.uint32(8)).astype(np.float32) * np.float32(2.0 ** -24) >= np.float32(0.5)
+    assert np.array_equal(y[-tail:].cpu().numpy() != 0, want)
+    r = philox4x32_10(31337, np.arange(0, tail // 4, dtype=np.uint64)).reshape(-1)
+    want = (r >> np.uint32(8)).astype(np.float32) * np.float32(2.0 ** -24) >= np.float32(0.5)
+    assert np.array_equal(y[:tail].cpu().numpy() != 0, want)
+
+
+@pytest.mark.gpu
+def test_nothing_is_written_behind_the_elements():
+    from yolo_from_scratch_amd import _lib as L
+    n = 1003
+    x = torch.randn(n, device=DEV).bfloat16()
+    y = torch.full((n + 64,), 3.0, device=DEV, dtype=torch.bfloat16)
+    s = torch.cuda.current_stream().cuda_stream
+    L.check(L.lib().yfs_dropout_fwd(x.data_ptr(), y.data_ptr(), n, 0.4, 0.1, 5, None, 1, s), "fwd")
+    assert (y[n:] == 3).all()
+    ref = y[:n].clone()
+    L.check(L.lib().yfs_dropout_fwd(x.data_ptr(), x.data_ptr(), n, 0.4, 0.1, 5, None, 1, s), "in place")
+    assert torch.equal(x, ref)
+
+
+@pytest.mark.gpu
+def test_seed_on_the_device_and_captured_graph():
+    """A graph whose seed lives on the GPU draws the mask of the seed that is there at each replay, forward and backward;
+    a seed that changes between forward and backward is refused."""
+    import yolo_from_scratch_amd as yfs
+    x = torch.randn(321, 65, device=DEV).bfloat16()
+    dy = torch.randn(321, 65, device=DEV).bfloat16()
+    seed = torch.tensor([(1 << 61) + 12345], device=DEV)
+    y, dx = _check(x, dy, 0.3, (1 << 61) + 12345, 0.1, seed_arg=seed)
+    negative = torch.tensor(-5, device=DEV)                       # the 64 bits are what counts
+    assert torch.equal(yfs.dropout(x, 0.3, negative), yfs.dropout(x, 0.3, 2 ** 64 - 5))
+    xg = x.clone().requires_grad_()
+    out = yfs.dropout(xg, 0.3, seed)
+    seed.add_(1)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, xg, dy)
+    del out        # a graph of the same leaf that was made outside a capture must not be alive while its backward is captured
+
+    def step():
+        out = yfs.dropout(xg, 0.3, seed, 0.1)
+        return out.detach(), torch.autograd.grad(out, xg, dy)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    seen = []
+    for k in range(4):
+        seed.fill_(1000 + k)
+        want = step()
+        got[0].fill_(7), got[1].fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
+        seen.append(got[0].clone())
+    assert not torch.equal(seen[0], seen[1])
+
+
+@pytest.mark.gpu
+def test_module():
+    import yolo_from_scratch_amd as yfs
+    m = yfs.HipDropout(0.25, slope=0.1)
+    x = torch.randn(64, 1000, device=DEV, requires_grad=True)
+    torch.manual_seed(1)
+    a = m(x)
+    b = m(x)
+    torch.manual_seed(1)
+    assert torch.equal(m(x), a) and not torch.equal(a, b)
+    assert abs(float((a == 0).float().mean()) - 0.25) < 0.01
+    (ga,) = torch.autograd.grad(a.sum(), x)
+    assert torch.equal(ga == 0, a == 0)
+    m.eval()
+    assert torch.equal(m(x), torch.nn.functional.leaky_relu(x, 0.1))
+    plain = yfs.HipDropout(0.5).eval()
+    assert plain(x) is x

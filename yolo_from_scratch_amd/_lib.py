@@ -27,10 +27,31 @@ def lib():
                      "yfs_conv2d_wgrad_workspace_bytes", "yfs_sumsq_workspace_bytes",
                      "yfs_conv2d_fwd_workspace_bytes", "yfs_conv2d_dgrad_workspace_bytes",
                      "yfs_conv2d_stem_wgrad_workspace_bytes", "yfs_single_box_loss_workspace_bytes",
-                     "yfs_mask_to_boxes_workspace_bytes"):
+                     "yfs_mask_to_boxes_workspace_bytes", "yfs_layer_norm_bwd_workspace_bytes"):
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = ctypes.c_size_t
+        _declare(_lib)
     return _lib
+
+
+# Entry points whose calls are short enough that ctypes' per-argument objects would show: their argument types are declared
+# once, so plain integers (data_ptr(), sizes, the raw stream) are passed as they are.  p pointer, l int64, z size_t, i int,
+# f float, u uint64.
+_SIGNATURES = {
+    "yfs_layer_norm_fwd": "plppppp" "ll" "fi" "p",
+    "yfs_layer_norm_bwd": "plpl" "ppp" "ppp" "ll" "i" "pz" "p",
+    "yfs_layer_norm_bwd_workspace_bytes": "lli",
+    "yfs_dropout_fwd": "ppl" "ff" "u" "p" "i" "p",
+    "yfs_dropout_bwd": "pppl" "ff" "u" "p" "i" "p",
+}
+_TYPES = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "z": ctypes.c_size_t, "i": ctypes.c_int, "f": ctypes.c_float,
+          "u": ctypes.c_uint64}
+
+
+def _declare(handle):
+    for name, sig in _SIGNATURES.items():
+        if hasattr(handle, name):
+            getattr(handle, name).argtypes = [_TYPES[c] for c in sig]
 
 
 KNOBS = {"igemm_tile": 0, "wgrad_tile": 1, "wgrad_splits": 2, "nms_fused": 3, "stem_kernel": 4, "igemm_persist": 5}     # include/yfs.h: yfs_knob_id
@@ -70,6 +91,38 @@ def ptr(t):
 
 def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # include/yfs.h: yfs_dtype
+
+
+class on_device:
+    """Context of a call on the tensors' own device, whichever device is current: gives the raw handle of that device's
+    current stream.  The tensors (None allowed) have to be on one GPU."""
+    __slots__ = ("index", "before")
+
+    def __init__(self, what, *tensors):
+        self.index = -1
+        for t in tensors:
+            if t is None:
+                continue
+            index = t.get_device()
+            if index < 0:
+                require_cuda(t)
+            if self.index >= 0 and index != self.index:
+                raise YfsError(f"{what}: tensors on devices {self.index} and {index}")
+            self.index = index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+        return False
 
 
 def require_cuda(*tensors):

@@ -1,0 +1,90 @@
+// Dropout from a counter-based generator, with the LeakyReLU in front of it: no mask is stored, the backward pass draws the
+// same numbers again.
+//   element e of the tensor in row-major order is kept iff (philox4x32_10(key = seed, counter = e / 4)[e % 4] >> 8) 2^-24 >= p
+//   y = keep ? leaky(x) / (1 - p) : 0          dx = keep ? dy / (1 - p) (y > 0 ? 1 : slope) : 0
+// (the rule of yfs_fc_epilogue_fwd_bf16: the same seed and p keep the same elements there).
+// (r >> 8) 2^-24 >= p  <=>  r >= ceil(p 2^24) 2^8, a comparison of whole numbers prepared on the host.
+#include "yfs_common.h"
+#include "yfs_vec.h"
+#include <math.h>
+
+namespace {
+constexpr int kThreads = 256;
+
+struct DropArgs {
+    const void *in, *y;          // x, or dy and (with a slope) y
+    void* out;
+    long long n;
+    unsigned long long seed;
+    const long long* seed_dev;   // overrides seed when not NULL
+    unsigned thr;                // kept iff r >= thr
+    int none;                    // p == 1: nothing is kept
+    float scale, slope;
+};
+
+template <typename T, bool BWD, bool ACT>
+__global__ void __launch_bounds__(kThreads) dropout_kernel(DropArgs g) {
+    constexpr int VE = 16 / sizeof(T);
+    const unsigned long long seed = g.seed_dev ? (unsigned long long)*g.seed_dev : g.seed;
+    for (long long id = (long long)blockIdx.x * kThreads + threadIdx.x; id * VE < g.n; id += (long long)gridDim.x * kThreads) {
+        const long long e = id * VE, left = g.n - e;
+        float v[VE], yv[VE];
+        load_vec((const T*)g.in + e, left, v);
+        if (BWD && ACT) load_vec((const T*)g.y + e, left, yv);
+#pragma unroll
+        for (int q = 0; q < VE / 4; ++q) {
+            unsigned r[4];
+            yfs_philox4(seed, (unsigned long long)(e / 4 + q), r);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = q * 4 + j;
+                float t = v[k];
+                if (ACT) t = (BWD ? yv[k] > 0.0f : t > 0.0f) ? t : t * g.slope;
+                v[k] = r[j] >= g.thr && !g.none ? t * g.scale : 0.0f;   // a select: NaN and Inf in dropped places leave nothing
+            }
+        }
+        store_vec((T*)g.out + e, left, v);
+    }
+}
+
+template <bool BWD, bool ACT>
+int launch(const DropArgs& g, int dtype, hipStream_t s) {
+    const long long vec = dtype == YFS_F32 ? 4 : 8;
+    long long nb = yfs_cdiv(yfs_cdiv(g.n, vec), kThreads);
+    if (nb > (1 << 20)) nb = 1 << 20;
+    const dim3 grid((unsigned)nb);
+    if (dtype == YFS_F32) dropout_kernel<float, BWD, ACT><<<grid, kThreads, 0, s>>>(g);
+    else if (dtype == YFS_BF16) dropout_kernel<__bf16, BWD, ACT><<<grid, kThreads, 0, s>>>(g);
+    else dropout_kernel<_Float16, BWD, ACT><<<grid, kThreads, 0, s>>>(g);
+    YFS_CHECK_LAUNCH("dropout_kernel");
+    return YFS_OK;
+}
+
+int run(const char* name, bool bwd, const void* in, const void* y, void* out, int64_t n, float p, float slope, uint64_t seed,
+        const int64_t* seed_dev, int dtype, void* stream) {
+    YFS_REQUIRE(in && out, YFS_ERR_INVALID_ARG, "%s: null pointer", name);
+    YFS_REQUIRE(n > 0, YFS_ERR_INVALID_ARG, "%s: n must be positive (got %lld)", name, (long long)n);
+    YFS_REQUIRE(p >= 0.0f && p <= 1.0f, YFS_ERR_INVALID_ARG, "%s: p %g not in [0, 1]", name, p);
+    YFS_REQUIRE(slope >= 0.0f && slope <= 1.0f, YFS_ERR_INVALID_ARG, "%s: slope %g not in [0, 1]", name, slope);
+    YFS_REQUIRE(dtype == YFS_F32 || dtype == YFS_BF16 || dtype == YFS_F16, YFS_ERR_UNSUPPORTED, "%s: unknown dtype %d", name, dtype);
+    const bool act = slope != 1.0f;
+    YFS_REQUIRE(!bwd || !act || y, YFS_ERR_INVALID_ARG, "%s: the gradient of an activation needs y", name);
+    DropArgs g = {in, y, out, n, seed, (const long long*)seed_dev, 0u, p >= 1.0f, 0.0f, slope};
+    const double t = ceil((double)p * 16777216.0);
+    g.thr = g.none ? 0xFFFFFFFFu : (unsigned)t << 8;
+    g.scale = g.none ? 0.0f : (float)(1.0 / (1.0 - (double)p));
+    hipStream_t s = (hipStream_t)stream;
+    if (bwd) return act ? launch<true, true>(g, dtype, s) : launch<true, false>(g, dtype, s);
+    return act ? launch<false, true>(g, dtype, s) : launch<false, false>(g, dtype, s);
+}
+}  // namespace
+
+YFS_API int yfs_dropout_fwd(const void* x, void* y, int64_t n, float p, float slope, uint64_t seed, const int64_t* seed_dev,
+                            int dtype, void* stream) {
+    return run("yfs_dropout_fwd", false, x, nullptr, y, n, p, slope, seed, seed_dev, dtype, stream);
+}
+
+YFS_API int yfs_dropout_bwd(const void* dy, const void* y, void* dx, int64_t n, float p, float slope, uint64_t seed,
+                            const int64_t* seed_dev, int dtype, void* stream) {
+    return run("yfs_dropout_bwd", true, dy, y, dx, n, p, slope, seed, seed_dev, dtype, stream);
+}

@@ -11,28 +11,6 @@ typedef __bf16 bf16_t;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 constexpr int kThreads = 256;
 
-// Philox4x32-10 (Salmon et al., SC'11): counter = (element group, 0, 0, 0), key = seed.
-__device__ __forceinline__ void philox_round(unsigned (&c)[4], unsigned k0, unsigned k1) {
-    const unsigned long long p0 = 0xD2511F53ull * c[0], p1 = 0xCD9E8D57ull * c[2];
-    const unsigned h0 = (unsigned)(p0 >> 32), l0 = (unsigned)p0, h1 = (unsigned)(p1 >> 32), l1 = (unsigned)p1;
-    c[0] = h1 ^ c[1] ^ k0;
-    c[1] = l1;
-    c[2] = h0 ^ c[3] ^ k1;
-    c[3] = l0;
-}
-__device__ __forceinline__ void philox4(unsigned long long seed, unsigned long long ctr, unsigned (&out)[4]) {
-    unsigned c[4] = {(unsigned)ctr, (unsigned)(ctr >> 32), 0u, 0u};
-    unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
-#pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        philox_round(c, k0, k1);
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = c[i];
-}
-
 // one thread = 8 consecutive outputs of one row
 __global__ void __launch_bounds__(kThreads) fc_epilogue_fwd_kernel(const float* __restrict__ partial, int splits,
                                                                    const float* __restrict__ bias, bf16_t* __restrict__ y,
@@ -56,8 +34,8 @@ __global__ void __launch_bounds__(kThreads) fc_epilogue_fwd_kernel(const float* 
         unsigned r[8];
         if (p_drop > 0.0f) {
             unsigned r0[4], r1[4];
-            philox4(seed, (unsigned long long)id * 2, r0);
-            philox4(seed, (unsigned long long)id * 2 + 1, r1);
+            yfs_philox4(seed, (unsigned long long)id * 2, r0);
+            yfs_philox4(seed, (unsigned long long)id * 2 + 1, r1);
 #pragma unroll
             for (int j = 0; j < 4; ++j) { r[j] = r0[j]; r[4 + j] = r1[j]; }
         }

@@ -42,6 +42,28 @@ __device__ __forceinline__ float yfs_wave_sum(float v) {
     return v;   // lane 0 holds the sum, fixed reduction tree => deterministic
 }
 
+// Philox4x32-10 (Salmon et al., SC'11): counter = (element group, 0, 0, 0), key = seed.
+__device__ __forceinline__ void yfs_philox_round(unsigned (&c)[4], unsigned k0, unsigned k1) {
+    const unsigned long long p0 = 0xD2511F53ull * c[0], p1 = 0xCD9E8D57ull * c[2];
+    const unsigned h0 = (unsigned)(p0 >> 32), l0 = (unsigned)p0, h1 = (unsigned)(p1 >> 32), l1 = (unsigned)p1;
+    c[0] = h1 ^ c[1] ^ k0;
+    c[1] = l1;
+    c[2] = h0 ^ c[3] ^ k1;
+    c[3] = l0;
+}
+__device__ __forceinline__ void yfs_philox4(unsigned long long seed, unsigned long long ctr, unsigned (&out)[4]) {
+    unsigned c[4] = {(unsigned)ctr, (unsigned)(ctr >> 32), 0u, 0u};
+    unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        yfs_philox_round(c, k0, k1);
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = c[i];
+}
+
 // Stage the global floats [src, src+len) into LDS asynchronously (global -> LDS DMA, `buffer_load ... lds`):
 // one wave-instruction moves 1 KiB (lane i lands at chunk base + 16 i), no staging registers, and every
 // instruction of the copy is issued before anything is waited for.  A per-thread `load; wait; ds_write` loop
