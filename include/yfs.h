@@ -349,6 +349,37 @@ int yfs_anchor_assign_f32(const float *wh, int64_t n, const float *anchors, int 
 
 typedef enum { YFS_F32 = 0, YFS_BF16 = 1, YFS_F16 = 2 } yfs_dtype;
 
+/* Matrix product in 8-bit floating point with a scale for each block of 128.
+ * A block's scale is the smallest power of two s = 2^e, e >= -127, with max|x| <= 448 s over the block's finite elements (1
+ * for a block of zeros), kept as the byte e + 127 (E8M0); q = x / s as e4m3, to nearest, ties to even (Inf, NaN -> NaN).
+ *   weights:                 q [N, pad(K)], scale [ceil(N/128), ceil(K/128)]: one for each 128 x 128
+ *   activations, gradients:  q [M, pad(K)], one for each row and 128 columns, in "packed" order: row r of block kb at byte
+ *                            (kb * G + r / 64) * 64 + (r % 16) * 4 + (r % 64) / 16 with G = 4 * ceil(M / 256)
+ * pad(n) = n rounded up to 128 (zeros behind the last column); sizes up to 2^23 - 256; q arrays and packed scales 16-byte
+ * aligned.  x and w: `dtype` elements, ld elements from row to row, any alignment.
+ * yfs_fp8_quantize_weight: qt / scale_t (both or neither NULL) = the transpose, [K, pad(N)] and [ceil(K/128), ceil(N/128)].
+ * yfs_fp8_quantize_rows: q / scale = x by rows; qt / scale_t = x^T by rows (blocks of 128 rows of x), [K, pad(M)]; either pair
+ *   may be NULL.  colsum (may be NULL) [ceil(M/128), K]: sums of x over each 128 rows; yfs_fp8_colsum adds them up in order. */
+int yfs_fp8_quantize_weight(const void *w, int dtype, int64_t ld, int64_t N, int64_t K, void *q, void *scale, void *qt,
+                            void *scale_t, void *stream);
+size_t yfs_fp8_packed_scale_bytes(int64_t rows, int64_t cols);
+int yfs_fp8_quantize_rows(const void *x, int dtype, int64_t ld, int64_t M, int64_t K, void *q, void *scale, void *qt,
+                          void *scale_t, float *colsum, void *stream);
+int yfs_fp8_colsum(const float *part, int64_t tiles, int64_t K, float *out, int accumulate, void *stream);
+/* out [M, N] = leaky(a b^T + bias): a [M, K] with packed row scales, b [N, K] with packed row scales (b_row_scales != 0) or
+ * 128 x 128 scales.  bias [N] fp32 or NULL; slope 1 = no activation.  out_dtype fp32: full fp32 sums, accumulate != 0 adds to
+ * what is there (before the activation); bf16 / fp16: the e4m3 matrix instructions, whose sums over one block keep about 16
+ * bits behind the largest product. */
+size_t yfs_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int yfs_fp8_gemm(const void *aq, const void *a_scale, const void *bq, const void *b_scale, int b_row_scales, const float *bias,
+                 void *out, int out_dtype, int64_t M, int64_t N, int64_t K, float slope, int accumulate, void *workspace,
+                 size_t workspace_bytes, void *stream);
+/* The serving form: x [M, K] in `x_dtype` is quantised by rows in the workspace and multiplied by a stored weight. */
+size_t yfs_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int yfs_fp8_matmul(const void *x, int x_dtype, int64_t ld, const void *wq, const void *w_scale, const float *bias, void *y,
+                   int out_dtype, int64_t M, int64_t N, int64_t K, float slope, void *workspace, size_t workspace_bytes,
+                   void *stream);
+
 /* Layer norm over the last axis: y = (x - mu) / sqrt(v + eps) * w + b with the row's mean mu and biased variance v, all in
  * fp32 with one rounding at the end.  x [rows, cols] with x_stride elements from row to row (0: one row for all), y [rows,
  * cols] dense, both `dtype`; w, b [cols] fp32 or NULL (ones / zeros); mean, rstd [rows] fp32 or NULL: what the backward

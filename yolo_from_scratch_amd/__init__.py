@@ -12,3 +12,5 @@ from .data import mask_to_boxes, box_to_xywh_norm, largest_box, mask_to_target_b
 from .conv_ops import release_workspaces  # noqa: F401,E402
 from .norm_ops import layer_norm, HipLayerNorm  # noqa: F401,E402
 from .drop_ops import dropout, HipDropout  # noqa: F401,E402
+from .fp8_ops import (Fp8Tensor, quantize_fp8, fp8_matmul, fp8_linear, Fp8Linear, FrozenFp8Linear,  # noqa: F401,E402
+                      freeze_fp8)

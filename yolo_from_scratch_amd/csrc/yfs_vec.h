@@ -44,3 +44,17 @@ __device__ __forceinline__ void load_vec_or(const float* p, long long c, long lo
         for (int j = 0; j < VE; ++j) v[j] = j < n ? p[c + j] : 0.0f;
     }
 }
+
+// 8 elements of any of the three types; n = elements left in the row
+template <typename T>
+__device__ __forceinline__ void load_vec8(const T* p, long long n, float (&v)[8]) {
+    T t[8];
+    if (n >= 8) {
+        __builtin_memcpy(t, p, 8 * sizeof(T));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)t[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.0f;
+    }
+}

@@ -1,0 +1,303 @@
+"""Matrix product in 8-bit floating point with a scale for each block of 128 (csrc/fp8_kernels.hip, include/yfs.h: yfs_fp8_*).
+
+What the head's linear layers (yolo_toy_regressor_torch.py:259, :262) multiply in 16 bits, in 8: weights are e4m3 with a
+power-of-two scale for each 128 x 128 block, activations and gradients with one for each row and 128 columns.
+
+* serving: ``quantize_fp8`` once, then ``fp8_matmul(x, w)`` per call, or ``FrozenFp8Linear`` / ``freeze_fp8(model)``;
+* training: ``fp8_linear(x, weight, bias)`` / ``Fp8Linear``: 32-bit master weights, three 8-bit products
+  (y = x W^T, dx = dy W, dW = dy^T x), each operand scaled along the axis that its product sums over.
+
+A block's scale is the smallest power of two s >= 2^-127 with max|x| <= 448 s over its finite elements (1 for zeros);
+x / s is rounded to nearest, ties to even.  NaN and infinities become NaN, without touching the scale.
+"""
+import torch
+import torch.nn as nn
+
+from . import _lib as L
+
+BLOCK = 128
+
+
+def _pad(n):
+    return (n + BLOCK - 1) // BLOCK * BLOCK
+
+
+class Fp8Tensor:
+    """A weight [n, k] in 8 bits: ``data`` float8_e4m3fn [n, k rounded up to 128] (zeros behind k), ``scale`` float8_e8m0fnu
+    [ceil(n / 128), ceil(k / 128)]: the values are data * scale, block by block."""
+    __slots__ = ("data", "scale", "k")
+
+    def __init__(self, data, scale, k, block=(BLOCK, BLOCK)):
+        if tuple(block) != (BLOCK, BLOCK):
+            raise L.YfsError(f"Fp8Tensor: blocks are {BLOCK} x {BLOCK}, got {tuple(block)}")
+        if data.dim() != 2 or data.dtype != torch.float8_e4m3fn or not 0 < k <= data.shape[1] or data.shape[1] != _pad(k):
+            raise L.YfsError(f"Fp8Tensor: data must be float8_e4m3fn [n, {_pad(k)}] for k = {k}, got {data.dtype} {tuple(data.shape)}")
+        want = (_pad(data.shape[0]) // BLOCK, data.shape[1] // BLOCK)
+        if tuple(scale.shape) != want or scale.dtype != torch.float8_e8m0fnu:
+            raise L.YfsError(f"Fp8Tensor: scale must be float8_e8m0fnu {want}, got {scale.dtype} {tuple(scale.shape)}")
+        if not data.is_contiguous() or not scale.is_contiguous() or data.data_ptr() % 16:
+            raise L.YfsError("Fp8Tensor: data and scale must be contiguous, data 16-byte aligned")
+        self.data, self.scale, self.k = data, scale, k
+
+    @property
+    def shape(self):
+        return torch.Size((self.data.shape[0], self.k))
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def dequantize(self):
+        """The fp32 values [n, k]."""
+        s = self.scale.float().repeat_interleave(BLOCK, 0)[: self.data.shape[0]].repeat_interleave(BLOCK, 1)
+        return (self.data.float() * s)[:, : self.k].contiguous()
+
+    def __repr__(self):
+        return f"Fp8Tensor({tuple(self.shape)}, device={self.device})"
+
+
+def _matrix(t, what):
+    """[..., k] -> rows with unit stride inside a row, the count of rows and the row stride."""
+    if t.dtype not in L.DTYPES:
+        raise L.YfsError(f"{what}: expected fp32, bf16 or fp16, got {t.dtype}")
+    k = t.shape[-1]
+    if t.dim() == 1:
+        t = t.unsqueeze(0)
+    if t.dim() != 2 or (k > 1 and t.stride(1) != 1):
+        t = t.contiguous().view(-1, k)
+    return t, t.shape[0], t.stride(0)
+
+
+def _p(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _check_weight(w):
+    if w.dim() != 2 or w.shape[0] == 0 or w.shape[1] == 0 or w.dtype not in L.DTYPES:
+        raise L.YfsError(f"quantize_fp8: expected a non-empty fp32, bf16 or fp16 matrix, got {w.dtype} {tuple(w.shape)}")
+
+
+def _quantize_weight(w, transposed):
+    """-> (data, scale) and, when asked, (data, scale) of the transpose: the same bytes, block by block."""
+    w2, n, ld = _matrix(w.detach(), "quantize_fp8")
+    k, dev = w2.shape[1], w2.device
+    nb, kb = _pad(n) // BLOCK, _pad(k) // BLOCK
+    q = torch.empty(n, kb * BLOCK, device=dev, dtype=torch.float8_e4m3fn)
+    s = torch.empty(nb, kb, device=dev, dtype=torch.float8_e8m0fnu)
+    qt = torch.empty(k, nb * BLOCK, device=dev, dtype=torch.float8_e4m3fn) if transposed else None
+    st = torch.empty(kb, nb, device=dev, dtype=torch.float8_e8m0fnu) if transposed else None
+    with L.on_device("quantize_fp8", w2) as stream:
+        L.check(L.lib().yfs_fp8_quantize_weight(w2.data_ptr(), L.DTYPES[w2.dtype], ld, n, k, q.data_ptr(), s.data_ptr(), _p(qt),
+                                                _p(st), stream), "yfs_fp8_quantize_weight")
+    return q, s, qt, st
+
+
+@torch.no_grad()
+def quantize_fp8(w):
+    """A weight matrix [n, k] (fp32, bf16 or fp16, rows with any stride) as ``Fp8Tensor``."""
+    _check_weight(w)
+    L.require_cuda(w)
+    q, s, _, _ = _quantize_weight(w, False)
+    return Fp8Tensor(q, s, w.shape[1])
+
+
+def _bias(b, n, what):
+    if b is None:
+        return None
+    if b.dim() != 1 or b.shape[0] != n or not b.is_floating_point():
+        raise L.YfsError(f"{what}: bias must be floating point [{n}], got {b.dtype} {tuple(b.shape)}")
+    b = b.detach()
+    if b.dtype != torch.float32:
+        b = b.float()
+    return b if b.is_contiguous() else b.contiguous()
+
+
+def _slope(slope, what):
+    slope = 1.0 if slope is None else float(slope)
+    if not 0.0 <= slope <= 1.0:
+        raise L.YfsError(f"{what}: slope must lie in [0, 1], got {slope}")
+    return slope
+
+
+@torch.no_grad()
+def fp8_matmul(x, w, bias=None, slope=None, out_dtype=None):
+    """y [..., n] = leaky(Q(x) W^T + bias) for x [..., k] (fp32, bf16 or fp16; quantised by rows inside the call) and an
+    ``Fp8Tensor`` w [n, k].  ``slope``: of a LeakyReLU behind the product (None: none).  ``out_dtype``: fp32, bf16 or fp16
+    (default: x's).  Sums are fp32 when the output is; towards 16 bits the 8-bit matrix instruction sums a block of 128 with
+    about 16 bits behind its largest product, 1 / 64 of the output's own rounding.  Not differentiable: see ``fp8_linear``."""
+    if not isinstance(w, Fp8Tensor):
+        raise L.YfsError(f"fp8_matmul: w must be an Fp8Tensor (quantize_fp8), got {type(w).__name__}")
+    if x.dim() == 0 or x.shape[-1] != w.k:
+        raise L.YfsError(f"fp8_matmul: x [..., {w.k}] expected, got {tuple(x.shape)}")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in L.DTYPES:
+        raise L.YfsError(f"fp8_matmul: out_dtype must be fp32, bf16 or fp16, got {out_dtype}")
+    n, slope = w.data.shape[0], _slope(slope, "fp8_matmul")
+    x2, m, ld = _matrix(x.detach(), "fp8_matmul")
+    b = _bias(bias, n, "fp8_matmul")
+    L.require_cuda(x, w.data, w.scale, bias)
+    y = torch.empty(x.shape[:-1] + (n,), device=x.device, dtype=out_dtype)
+    if m == 0:
+        return y
+    lib = L.lib()
+    nbytes = lib.yfs_fp8_matmul_workspace_bytes(m, n, w.k)
+    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+    with L.on_device("fp8_matmul", x2, w.data, w.scale, b) as stream:
+        L.check(lib.yfs_fp8_matmul(x2.data_ptr(), L.DTYPES[x2.dtype], ld, w.data.data_ptr(), w.scale.data_ptr(), _p(b), y.data_ptr(),
+                                   L.DTYPES[out_dtype], m, n, w.k, slope, ws.data_ptr(), nbytes, stream), "yfs_fp8_matmul")
+    return y
+
+
+def _quantize_rows(x, rows, cols, colsum=False):
+    """x [m, k] -> (q, scales) by rows of 128 columns and (q, scales) of the transpose by 128 rows, either may be left out, and
+    the sums of x over tiles of 128 rows."""
+    x2, m, ld = _matrix(x.detach(), "fp8_linear")
+    k, dev, lib = x2.shape[1], x2.device, L.lib()
+    e4, u8 = torch.float8_e4m3fn, torch.uint8
+    q = torch.empty(m, _pad(k), device=dev, dtype=e4) if rows else None
+    s = torch.empty(lib.yfs_fp8_packed_scale_bytes(m, k), device=dev, dtype=u8) if rows else None
+    qt = torch.empty(k, _pad(m), device=dev, dtype=e4) if cols else None
+    st = torch.empty(lib.yfs_fp8_packed_scale_bytes(k, m), device=dev, dtype=u8) if cols else None
+    cs = torch.empty(_pad(m) // BLOCK, k, device=dev, dtype=torch.float32) if colsum else None
+    with L.on_device("fp8_linear", x2) as stream:
+        L.check(lib.yfs_fp8_quantize_rows(x2.data_ptr(), L.DTYPES[x2.dtype], ld, m, k, _p(q), _p(s), _p(qt), _p(st), _p(cs), stream),
+                "yfs_fp8_quantize_rows")
+    return q, s, qt, st, cs
+
+
+def _gemm(aq, a_s, bq, b_s, row_scales, bias, out, m, n, k, accumulate=False):
+    lib = L.lib()
+    nbytes = lib.yfs_fp8_gemm_workspace_bytes(m, n, k)
+    ws = torch.empty(nbytes, device=out.device, dtype=torch.uint8) if nbytes else None
+    with L.on_device("fp8_linear", aq, bq, bias, out) as stream:
+        L.check(lib.yfs_fp8_gemm(aq.data_ptr(), a_s.data_ptr(), bq.data_ptr(), b_s.data_ptr(), row_scales, _p(bias), out.data_ptr(),
+                                 L.DTYPES[out.dtype], m, n, k, 1.0, int(accumulate), _p(ws), nbytes, stream), "yfs_fp8_gemm")
+    return out
+
+
+class _Fp8LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        n, k = weight.shape
+        need_x, need_w, need_b = ctx.needs_input_grad
+        m = x.numel() // k
+        ctx.meta = (x.shape, x.dtype, m, n, k, bias.dtype if bias is not None else None)
+        ctx.wb = (weight, bias)          # for their gradient sinks; their values are not read again
+        y = torch.empty(x.shape[:-1] + (n,), device=x.device, dtype=x.dtype)
+        if m == 0:
+            ctx.save_for_backward(None, None, None, None)
+            return y
+        wq, ws, wqt, wst = _quantize_weight(weight, need_x)
+        xq, xs, xqt, xst, _ = _quantize_rows(x, True, need_w)
+        _gemm(xq, xs, wq, ws, 0, _bias(bias, n, "fp8_linear"), y, m, n, k)
+        # what the backward pass multiplies: the weight's blocks transposed, x's columns in blocks of 128 rows (8 bits each)
+        ctx.save_for_backward(wqt, wst, xqt, xst)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        from .train import write_grad
+        wqt, wst, xqt, xst = ctx.saved_tensors
+        shape, dtype, m, n, k, bias_dtype = ctx.meta
+        weight, bias = ctx.wb
+        need_x, need_w, need_b = ctx.needs_input_grad
+        dev = dy.device
+        if m == 0:
+            return (torch.empty(shape, device=dev, dtype=dtype) if need_x else None,
+                    torch.zeros_like(weight) if need_w else None, torch.zeros_like(bias) if need_b else None)
+        dy2 = _matrix(dy if dy.dtype in L.DTYPES else dy.to(dtype), "fp8_linear")[0]
+        dq, ds, dqt, dst, colsum = _quantize_rows(dy2, need_x, need_w, need_b) if (need_x or need_w) else (None,) * 5
+        dx = dw = db = None
+        if need_x:
+            dx = _gemm(dq, ds, wqt, wst, 0, None, torch.empty(shape, device=dev, dtype=dtype), m, k, n)
+
+        def put_w(sink, acc):
+            direct = sink is not None and sink.dtype == torch.float32 and sink.is_contiguous()
+            out = _gemm(dqt, dst, xqt, xst, 1, None, sink if direct else torch.empty(n, k, device=dev, dtype=torch.float32), n, k, m,
+                        acc and direct)
+            if sink is None:
+                return out if weight.dtype == torch.float32 else out.to(weight.dtype)
+            if not direct:
+                sink.add_(out) if acc else sink.copy_(out)
+
+        def put_b(sink, acc):
+            if colsum is None:
+                total = dy2.float().sum(0)
+            else:
+                direct = sink is not None and sink.dtype == torch.float32 and sink.is_contiguous()
+                total = sink if direct else torch.empty(n, device=dev, dtype=torch.float32)
+                with L.on_device("fp8_linear", colsum, total) as stream:
+                    L.check(L.lib().yfs_fp8_colsum(colsum.data_ptr(), colsum.shape[0], n, total.data_ptr(), int(acc and direct), stream),
+                            "yfs_fp8_colsum")
+                if direct:
+                    return None
+            if sink is None:
+                return total if bias_dtype == torch.float32 else total.to(bias_dtype)
+            sink.add_(total) if acc else sink.copy_(total)
+        if need_w:
+            dw = write_grad(weight, put_w)
+        if need_b:
+            db = write_grad(bias, put_b)
+        ctx.wb = None
+        return dx, dw, db
+
+
+def fp8_linear(x, weight, bias=None):
+    """y [..., n] = Q(x) Q(weight)^T + bias, differentiable, in x's dtype: x [..., k] and weight [n, k] fp32, bf16 or fp16.
+    The backward pass multiplies in 8 bits too: dx = Q(dy) Q(weight), dW = Q(dy^T) Q(x^T)^T (summed in fp32, as the bias's
+    gradient is); for it the transposed 8-bit weight and x are kept, not the 16-bit x."""
+    _check_weight(weight)
+    if x.dim() == 0 or x.shape[-1] != weight.shape[1] or x.dtype not in L.DTYPES:
+        raise L.YfsError(f"fp8_linear: x fp32, bf16 or fp16 [..., {weight.shape[1]}] expected, got {x.dtype} {tuple(x.shape)}")
+    _bias(bias, weight.shape[0], "fp8_linear")
+    L.require_cuda(x, weight, bias)
+    return _Fp8LinearFn.apply(x, weight, bias)
+
+
+class Fp8Linear(nn.Linear):
+    """nn.Linear (same parameter names and initialisation, fp32 master weights) whose three products run in 8 bits.  Takes
+    fp32, bf16 or fp16 rows and answers in bf16, as ``HipLinear`` does; its gradients go straight into FlatSGD's arena."""
+
+    def __init__(self, in_features, out_features, bias=True):
+        super().__init__(in_features, out_features, bias=bias)
+        self.weight._yfs_sink_capable = True
+        if bias:
+            self.bias._yfs_sink_capable = True
+
+    def forward(self, x):
+        return fp8_linear(x.to(torch.bfloat16), self.weight, self.bias)
+
+
+class FrozenFp8Linear(nn.Module):
+    """A linear layer for serving: 8-bit weights as buffers (a quarter of the fp32 bytes), bias, and the LeakyReLU(slope)
+    that follows (None: none).  Not trainable."""
+
+    def __init__(self, linear, slope=None):
+        super().__init__()
+        w = quantize_fp8(linear.weight)
+        self.out_features, self.in_features = w.shape
+        self.slope = slope
+        self.register_buffer("weight_data", w.data)
+        self.register_buffer("weight_scale", w.scale)
+        self.register_buffer("bias", linear.bias.detach().float().clone() if linear.bias is not None else None)
+
+    def forward(self, x):
+        w = Fp8Tensor(self.weight_data, self.weight_scale, self.in_features)
+        return fp8_matmul(x, w, self.bias, self.slope, torch.bfloat16)
+
+    def extra_repr(self):
+        return f"{self.in_features}, {self.out_features}, slope={self.slope}"
+
+
+def freeze_fp8(model):
+    """Replaces every linear layer of ``model`` (on the GPU) by its 8-bit form for serving, a fused LeakyReLU included, and
+    puts the model into eval mode.  In place; returns the model."""
+    from .model import HipLinear
+    from .train import bf16_shadow
+    for module in list(model.modules()):
+        for name, child in list(module.named_children()):
+            if isinstance(child, nn.Linear):
+                bf16_shadow(child.weight)          # a step that is still running on the weight is waited for
+                module._modules[name] = FrozenFp8Linear(child, child.fused_act if isinstance(child, HipLinear) else None)
+    return model.eval()
