@@ -213,9 +213,16 @@ def test_matmul(m, n, k):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,n,k", [(1, 4096, 50176), (64, 512, 50176), (1500, 1300, 1111), (700, 2048, 4096)])
-def test_matmul_large_against_fp64_on_the_gpu(m, n, k):
+@pytest.mark.parametrize("m,n,k,kernel", [(1, 4096, 50176, "fp8_rows_kernel"), (3, 40, 50176, "fp8_rows_kernel"),
+                                          (16, 1470, 4096, "fp8_rows_kernel"), (16, 512, 50176, "fp8_gemm_kernel<64"),
+                                          (64, 512, 50176, "fp8_gemm_kernel<64"), (1500, 1300, 1111, "fp8_gemm_kernel<128"),
+                                          (700, 2048, 4096, "fp8_gemm_kernel<128"), (4099, 4101, 640, "fp8_gemm8_kernel"),
+                                          (4352, 4096, 768, "fp8_gemm8_kernel"), (2100, 8300, 515, "fp8_gemm8_kernel"),
+                                          (8192, 2304, 2048, "fp8_gemm8_kernel")])
+def test_matmul_large_against_fp64_on_the_gpu(m, n, k, kernel):
+    """Every kernel the size rule chooses, at ragged sizes and odd counts of blocks."""
     import yolo_from_scratch_amd as yfs
+    from yolo_from_scratch_amd import _lib as L
     g = torch.Generator(DEV).manual_seed(m + n)
     x = torch.randn(m, k, device=DEV, generator=g).bfloat16()
     w = torch.randn(n, k, device=DEV, generator=g) / k ** 0.5
@@ -228,6 +235,7 @@ def test_matmul_large_against_fp64_on_the_gpu(m, n, k):
     assert ((f32 - ref).abs() <= (96 + k / 32) * 2.0 ** -24 * mag).all()
     assert float((f32 - ref).norm() / ref.norm()) < 2e-6
     b16 = yfs.fp8_matmul(x, wq).double()
+    assert L.last_kernel().startswith(kernel)
     assert float((b16 - ref).norm() / ref.norm()) < 2.0 ** -8      # every value within half a step, 2^-8 of it at most
     assert float((b16 - f32.bfloat16().double()).norm() / ref.norm()) < 2.0 ** -9
 

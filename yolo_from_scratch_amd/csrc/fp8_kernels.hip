@@ -160,6 +160,27 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(QuantArgs g) {
     }
 }
 
+// By rows alone: 16 lanes x 8 elements per block, blocks of a row next to each other.
+template <typename T>
+__global__ void __launch_bounds__(256) quant_rows_kernel(QuantArgs g) {
+    const long long kblocks = (g.K + 127) >> 7, total = g.M * kblocks;
+    const int l = threadIdx.x & 15;
+    for (long long id = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); id < total; id += (long long)gridDim.x * 16) {
+        const long long m = id / kblocks, kb = id - m * kblocks, k = kb * 128 + l * 8;
+        float v[8], a = 0.0f;
+        load_vec8((const T*)g.x + m * g.ld + k, g.K - k, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(v[j]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+        const int e = scale_exponent(a);
+        if (l == 0) g.s[packed_at(m, kb, g.groups)] = (unsigned char)(e + 127);
+        const float f = pow2(-e);
+        *reinterpret_cast<uint2*>(g.q + m * kblocks * 128 + k) =
+            make_uint2(pack4(v[0] * f, v[1] * f, v[2] * f, v[3] * f), pack4(v[4] * f, v[5] * f, v[6] * f, v[7] * f));
+    }
+}
+
 // sums over the tiles of quant_tile_kernel's colsum, in tile order
 __global__ void __launch_bounds__(256) colsum_kernel(const float* __restrict__ part, long long tiles, long long K,
                                                      float* __restrict__ out, int accumulate) {
@@ -168,6 +189,16 @@ __global__ void __launch_bounds__(256) colsum_kernel(const float* __restrict__ p
     float s = 0.0f;
     for (long long t = 0; t < tiles; ++t) s += part[t * K + k];
     out[k] = accumulate ? out[k] + s : s;
+}
+
+int quantize_rows_only(const QuantArgs& g, int dtype, hipStream_t s) {
+    const long long nb = yfs_cdiv(g.M * yfs_cdiv(g.K, 128), 16);
+    const dim3 grid((unsigned)(nb < 16384 ? nb : 16384));
+    if (dtype == YFS_F32) quant_rows_kernel<float><<<grid, 256, 0, s>>>(g);
+    else if (dtype == YFS_BF16) quant_rows_kernel<bf16_t><<<grid, 256, 0, s>>>(g);
+    else quant_rows_kernel<_Float16><<<grid, 256, 0, s>>>(g);
+    YFS_CHECK_LAUNCH("quant_rows_kernel");
+    return YFS_OK;
 }
 
 template <bool BLOCK, bool ROWQ, bool COLQ>
@@ -243,17 +274,47 @@ __device__ __forceinline__ void store4(const GemmArgs& g, long long m, long long
     }
 }
 
-// out tile of (WM FM 16) x (WN FN 16), a wave FM x FN fragments of 16 x 16.  LDS holds two stages of the 128-byte rows of both
-// operands, 16-byte chunks swizzled by the row, filled by direct loads.  The operands' lanes hold 32 of a block's 128 k in an
-// order that is the same on both sides, which is all that the sum needs.  The b rows are the instruction's first operand, so
-// that a lane owns four neighbouring columns of one output row.
+__device__ __forceinline__ void store_part(const GemmArgs& g, int split, long long m, long long n, f32x4 v) {
+    float* o = g.part + ((long long)split * g.M + m) * g.N + n;
+    if (n + 4 <= g.N) __builtin_memcpy(o, &v, 16);
+    else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (n + r < g.N) o[r] = v[r];
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The exponent byte of a 128-row block of b at k-block kb, through the scalar unit (the aligned dword that holds it: same page):
+// no vector register, and nothing that the counted waits for vector loads would see.
+__device__ __forceinline__ int block_scale(const unsigned char* row, int kb) {
+    typedef const __attribute__((address_space(4))) unsigned* cptr;
+    const uintptr_t p = reinterpret_cast<uintptr_t>(row) + (uintptr_t)(unsigned)kb;
+    return (int)((*reinterpret_cast<cptr>(p & ~(uintptr_t)3) >> ((p & 3) * 8)) & 255u);
+}
+
+// out tile of (WM FM 16) x (WN FN 16), a wave FM x FN fragments of 16 x 16.  LDS holds a ring of S stages: the 128-byte rows of
+// both operands, 16-byte chunks swizzled by the row, and the row scales, filled by direct loads.  S - 1 stages are on their
+// way while one is multiplied; a stage is waited for by count (DPS loads per wave and stage, in order) and handed over with one
+// barrier per k-block.  The operands' lanes hold 32 of a block's 128 k in an order that is the same on both sides, which is all
+// that the sum needs.  The b rows are the instruction's first operand, so that a lane owns four neighbouring columns of one
+// output row.
 // EXACT: the e4m3 instructions sum a block's products with about 16 bits behind the largest (measured: 1.5e-5 relative
 // whatever K, 2^-16); where the output is fp32 the operands are widened in registers and multiplied by the bf16 instruction,
 // whose sums are full fp32.
-template <int FM, int FN, int WM, int WN, bool ROWB, bool EXACT, typename TO>
+template <int FM, int FN, int WM, int WN, int S, bool ROWB, bool EXACT, typename TO>
 __global__ void __launch_bounds__(64 * WM * WN) fp8_gemm_kernel(GemmArgs g) {
     constexpr int BM = WM * FM * 16, BN = WN * FN * 16, NW = WM * WN;
-    constexpr int STAGE = (BM + BN) * 128;
+    constexpr int TILE = (BM + BN) * 128, STAGE = TILE + NW * 256 * (ROWB ? 2 : 1);
+    constexpr int DPS = (BM + BN) / 8 / NW + (ROWB ? 2 : 1);
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && FM * 16 <= 64 && FN * 16 <= 64, "rows per wave");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int wm = wave / WN, wn = wave % WN;
@@ -267,12 +328,27 @@ __global__ void __launch_bounds__(64 * WM * WN) fp8_gemm_kernel(GemmArgs g) {
     const unsigned chunk = (unsigned)((lane & 7) ^ srow) * 16u;
     auto stage = [&](int kb, int buf) {   // rows outside the operands read as zeros
         unsigned char* base = smem + buf * STAGE;
-        for (int r = wave; r < BM / 8; r += NW)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (lds_ptr)(base + r * 1024), 16, (unsigned)((r * 8 + srow) * ld) + chunk,
-                                                     (unsigned)kb * 128u, 0, 0);
-        for (int r = wave; r < BN / 8; r += NW)
+        const unsigned so = (unsigned)kb * 128u;
+#pragma unroll
+        for (int i = 0; i < BM / 8 / NW; ++i) {
+            const int r = wave * (BM / 8 / NW) + i;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (lds_ptr)(base + r * 1024), 16, (unsigned)((r * 8 + srow) * ld) + chunk, so, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < BN / 8 / NW; ++i) {
+            const int r = wave * (BN / 8 / NW) + i;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb, (lds_ptr)(base + BM * 128 + r * 1024), 16,
-                                                     (unsigned)((r * 8 + srow) * ld) + chunk, (unsigned)kb * 128u, 0, 0);
+                                                     (unsigned)((r * 8 + srow) * ld) + chunk, so, 0, 0);
+        }
+        // each wave its own copy of the scales: 4 groups of 64 rows; groups behind the plane's end are not used
+        const long long ga = (long long)kb * g.groups_a + (m0 >> 6);
+        const __amdgpu_buffer_rsrc_t rs = rsrc(g.as + ga * 64, ((long long)g.kblocks * g.groups_a - ga) * 64);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(base + TILE + wave * 256), 4, (unsigned)lane * 4u, 0, 0, 0);
+        if (ROWB) {
+            const long long gb = (long long)kb * g.groups_b + (n0 >> 6);
+            const __amdgpu_buffer_rsrc_t rt = rsrc(g.bs + gb * 64, ((long long)g.kblocks * g.groups_b - gb) * 64);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rt, (lds_ptr)(base + TILE + (NW + wave) * 256), 4, (unsigned)lane * 4u, 0, 0, 0);
+        }
     };
     const int frow = lane & 15, fk = lane >> 4;
     auto fragment = [&](const unsigned char* base, int row) {
@@ -280,29 +356,36 @@ __global__ void __launch_bounds__(64 * WM * WN) fp8_gemm_kernel(GemmArgs g) {
         const i32x4 hi = *reinterpret_cast<const i32x4*>(base + row * 128 + (((4 + fk) ^ (row & 7)) * 16));
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
+    // scales of a wave's F fragments: the dword of its 64-row group, shifted down to its first fragment
+    auto scales = [&](const unsigned char* base, int row0) {
+        const int d = *reinterpret_cast<const int*>(base + (row0 >> 6) * 64 + frow * 4);
+        return (int)((unsigned)d >> ((row0 & 63) / 16 * 8));
+    };
+    const long long nb = (n0 + wn * FN * 16) >> 7, last = (g.N - 1) >> 7;
+    const unsigned char* const bsrow = ROWB ? nullptr : g.bs + (nb < last ? nb : last) * g.kblocks;
+    int sbn = ROWB ? 0 : block_scale(bsrow, kb0);
     f32x4 acc[FN][FM];
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-    stage(kb0, 0);
-    for (int kb = kb0; kb < kb1; ++kb) {
-        const int buf = (kb - kb0) & 1;
-        const int sa = *reinterpret_cast<const int*>(g.as + ((long long)kb * g.groups_a + ((m0 + wm * FM * 16) >> 6)) * 64 + frow * 4);
-        int sb;
-        if (ROWB) {
-            sb = *reinterpret_cast<const int*>(g.bs + ((long long)kb * g.groups_b + ((n0 + wn * FN * 16) >> 6)) * 64 + frow * 4);
-            if (FN == 2) sb = (wn & 1) ? (int)((unsigned)sb >> 16) : sb;
-        } else {
-            const long long nb = (n0 + wn * FN * 16) >> 7, last = (g.N - 1) >> 7;
-            sb = g.bs[(nb < last ? nb : last) * g.kblocks + kb];
-        }
-        yfs_stage_wait();
-        __syncthreads();
-        if (kb + 1 < kb1) stage(kb + 1, buf ^ 1);
+    const int nit = kb1 - kb0;
+#pragma unroll
+    for (int t = 0; t < S - 1; ++t)
+        if (t < nit) stage(kb0 + t, t);
+    int buf = 0, into = S - 1;
+    for (int t = 0; t < nit; ++t) {
+        if (t + S - 2 < nit) wait_vm<DPS * (S - 2)>(); else wait_vm<0>();
+        barrier();   // stage t is there for every wave; every wave has left the stage before it
+        if (t + S - 1 < nit) stage(kb0 + t + S - 1, into);
+        into = into + 1 == S ? 0 : into + 1;
         const unsigned char* ab = smem + buf * STAGE;
         const unsigned char* bb = ab + BM * 128;
+        buf = buf + 1 == S ? 0 : buf + 1;
+        const int sa = scales(ab + TILE + wave * 256, wm * FM * 16);
+        const int sb = ROWB ? scales(ab + TILE + (NW + wave) * 256, wn * FN * 16) : sbn;
+        if (!ROWB && t + 1 < nit) sbn = block_scale(bsrow, kb0 + t + 1);
         i32x8 fa[FM], fb[FN];
 #pragma unroll
         for (int j = 0; j < FM; ++j) fa[j] = fragment(ab, wm * FM * 16 + j * 16 + frow);
@@ -336,7 +419,6 @@ __global__ void __launch_bounds__(64 * WM * WN) fp8_gemm_kernel(GemmArgs g) {
             row(std::integral_constant<int, 2>());
             row(std::integral_constant<int, 3>());
         }
-        __syncthreads();
     }
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
@@ -346,12 +428,260 @@ __global__ void __launch_bounds__(64 * WM * WN) fp8_gemm_kernel(GemmArgs g) {
         for (int i = 0; i < FN; ++i) {
             const long long n = n0 + wn * FN * 16 + i * 16 + fk * 4;
             if (n >= g.N) continue;
-            if (g.splits > 1) {
-                float* o = g.part + ((long long)blockIdx.z * g.M + m) * g.N + n;
+            if (g.splits > 1) store_part(g, blockIdx.z, m, n, acc[i][j]);
+            else store4<TO>(g, m, n, acc[i][j]);
+        }
+    }
+}
+
+// Large products: 256 x 256 outputs, 8 waves as 2 (row halves of a half-tile) x 4, one workgroup per CU.  The schedule of the
+// convolutions' 8-wave kernel with 8-bit rows: a k-block is four half-tiles of 16 KiB (128 rows x 128 bytes: A0, A1, B0, B1),
+// LDS holds two k-blocks, and the two row halves run one barrier apart, so that on every SIMD one wave multiplies while its
+// partner reads fragments and sends loads:
+//   phase A: read B0, A0, B1 | send A1 of block t + 1                       | 16 products with A0
+//   phase B: read A1         | send B0, A0, B1 and the scales of block t + 2 | 16 products with A1
+// A half-tile is sent again one phase after its fragments were read, every wave having retired its reads (lgkmcnt 0) before the
+// phase's first barrier.  The only wait for loads is in phase B and leaves the seven just sent on their way.
+// A wave's 128 x 64 outputs are 128 accumulators; a fragment pair read from LDS feeds 4 (2) products of 32 cycles.
+constexpr int G8_HALF = 128 * 128, G8_BUF = 4 * G8_HALF, G8_SCALES = 2 * G8_BUF;
+constexpr int G8_LDS = G8_SCALES + 2 * 8 * 256;
+
+template <typename TO>
+__global__ void __launch_bounds__(512, 2) fp8_gemm8_kernel(GemmArgs g) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wm = wave >> 2, wn = wave & 3, frow = lane & 15, fk = lane >> 4;
+    // Workgroups go round the 8 XCDs: each XCD gets neighbouring tiles, in groups of 8 tile rows, so that the tiles that run on
+    // it at one time share their operands' rows in its L2
+    const int mt = (int)((g.M + 255) >> 8), nt = (int)((g.N + 255) >> 8), total = mt * nt;
+    const int q8 = total >> 3, r8 = total & 7, xcd = (int)blockIdx.x & 7;
+    const int id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + ((int)blockIdx.x >> 3);
+    const int grp = id / (8 * nt), in = id - grp * 8 * nt, high = mt - grp * 8 < 8 ? mt - grp * 8 : 8;
+    const int tn = in / high, tm = grp * 8 + in - tn * high;
+    const long long m0 = __builtin_amdgcn_readfirstlane(tm) * 256LL, n0 = __builtin_amdgcn_readfirstlane(tn) * 256LL;
+    const long long ld = (long long)g.kblocks * 128;
+    const int nit = g.kblocks;
+    const unsigned ra = (unsigned)((g.M - m0 < 256 ? g.M - m0 : 256) * ld), rb = (unsigned)((g.N - n0 < 256 ? g.N - n0 : 256) * ld);
+    const unsigned char *const pa = g.a + m0 * ld, *const pb = g.b + n0 * ld, *const ps = g.as + (m0 >> 6) * 64;
+    const int srow = lane >> 3;
+    const unsigned off0 = (unsigned)((wave * 16 + srow) * ld) + (unsigned)((lane & 7) ^ srow) * 16u, off8 = (unsigned)(8 * ld), half = (unsigned)(128 * ld);
+    // Rows outside the operands, and whole blocks behind the last one, read as zeros (a descriptor of no bytes): every pass of
+    // the loop sends the same loads, without a branch.
+    auto stage = [&](const unsigned char* p, unsigned bytes, int h, int slot, int kb, int buf) {
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p), 0, kb < nit ? (int)bytes : 0, 0x00020000);
+        unsigned off = off0;
+        asm volatile("" : "+v"(off));   // (four sums of a register and a scalar a phase instead of four registers all the way)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (n + r < g.N) o[r] = acc[i][j][r];
-            } else store4<TO>(g, m, n, acc[i][j]);
+        for (int i = 0; i < 2; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(smem + buf * G8_BUF + slot * G8_HALF + (wave * 2 + i) * 1024), 16,
+                                                     off + (unsigned)i * off8 + (unsigned)h * half, (unsigned)kb * 128u, 0, 0);
+    };
+    auto stage_scales = [&](int kb, int buf) {   // each wave its own copy of the 256 rows' bytes
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(ps + (long long)kb * g.groups_a * 64), 0,
+                                                                            kb < nit ? 256 : 0, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(smem + G8_SCALES + (buf * 8 + wave) * 256), 4, (unsigned)lane * 4u, 0, 0, 0);
+    };
+    const long long last = (g.N - 1) >> 7, nb = n0 >> 7;
+    const unsigned char *const bs0 = g.bs + nb * nit, *const bs1 = g.bs + (nb + 1 < last ? nb + 1 : last) * nit;
+    int s0 = block_scale(bs0, 0), s1 = block_scale(bs1, 0), s0n, s1n;
+
+    f32x4 acc[2][2][2][4];   // [A half][B half][fragment of B][fragment of A]
+#pragma unroll
+    for (int i = 0; i < 32; ++i) (&acc[0][0][0][0])[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    auto fragment = [&](const unsigned char* base, int row) {
+        const i32x4 lo = *reinterpret_cast<const i32x4*>(base + row * 128 + ((fk ^ (row & 7)) * 16));
+        const i32x4 hi = *reinterpret_cast<const i32x4*>(base + row * 128 + (((4 + fk) ^ (row & 7)) * 16));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    i32x8 fa[4], fb0[2], fb1[2];
+    auto read_a = [&](const unsigned char* hb) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) fa[b] = fragment(hb, wm * 64 + b * 16 + frow);
+    };
+    auto read_b = [&](const unsigned char* hb, i32x8 (&f)[2]) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) f[a] = fragment(hb, wn * 32 + a * 16 + frow);
+    };
+    auto products = [&](f32x4 (&c)[2][4], const i32x8 (&f)[2], int sb, int sa) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            c[a][0] = mfma_fp8<0, 0>(f[a], fa[0], c[a][0], sb, sa);
+            c[a][1] = mfma_fp8<0, 1>(f[a], fa[1], c[a][1], sb, sa);
+            c[a][2] = mfma_fp8<0, 2>(f[a], fa[2], c[a][2], sb, sa);
+            c[a][3] = mfma_fp8<0, 3>(f[a], fa[3], c[a][3], sb, sa);
+        }
+        __builtin_amdgcn_s_setprio(0);
+    };
+    auto lgkm0 = [&]() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+
+    stage(pb, rb, 0, 2, 0, 0);
+    stage(pb, rb, 1, 3, 0, 0);
+    stage(pa, ra, 0, 0, 0, 0);
+    stage(pa, ra, 1, 1, 0, 0);
+    stage_scales(0, 0);
+    stage(pb, rb, 0, 2, 1, 1);
+    stage(pa, ra, 0, 0, 1, 1);
+    stage(pb, rb, 1, 3, 1, 1);
+    stage_scales(1, 1);
+    wait_vm<7>();
+    auto block = [&](int t, auto buf_tag) {
+        constexpr int BUF = decltype(buf_tag)::value;
+        const unsigned char* tb = smem + BUF * G8_BUF;
+        read_b(tb + 2 * G8_HALF, fb0);
+        read_a(tb);
+        read_b(tb + 3 * G8_HALF, fb1);
+        const unsigned char* sp = smem + G8_SCALES + (BUF * 8 + wave) * 256 + frow * 4;
+        const int sa0 = *reinterpret_cast<const int*>(sp + wm * 64), sa1 = *reinterpret_cast<const int*>(sp + 128 + wm * 64);
+        const int tn = t + 1 < nit ? t + 1 : nit - 1;
+        s0n = block_scale(bs0, tn);
+        s1n = block_scale(bs1, tn);
+        stage(pa, ra, 1, 1, t + 1, BUF ^ 1);
+        lgkm0();
+        barrier();
+        products(acc[0][0], fb0, s0, sa0);
+        products(acc[0][1], fb1, s1, sa0);
+        barrier();
+        read_a(tb + G8_HALF);
+        stage(pb, rb, 0, 2, t + 2, BUF);
+        stage(pa, ra, 0, 0, t + 2, BUF);
+        stage(pb, rb, 1, 3, t + 2, BUF);
+        stage_scales(t + 2, BUF);
+        wait_vm<7>();
+        lgkm0();
+        barrier();
+        products(acc[1][1], fb1, s1, sa1);
+        products(acc[1][0], fb0, s0, sa1);
+        barrier();
+        s0 = s0n;
+        s1 = s1n;
+    };
+    barrier();
+    if (wm == 1) barrier();   // waves 4-7 run one barrier behind waves 0-3 from here on
+    for (int t = 0; t < nit; t += 2) {   // an odd count ends with a block of zeros
+        block(t, std::integral_constant<int, 0>());
+        block(t + 1, std::integral_constant<int, 1>());
+    }
+    if (wm == 0) barrier();
+    wait_vm<0>();
+#pragma unroll
+    for (int wh = 0; wh < 2; ++wh)
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            const long long n = n0 + wh * 128 + wn * 32 + a * 16 + fk * 4;
+            if (n >= g.N) continue;
+#pragma unroll
+            for (int ph = 0; ph < 2; ++ph)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const long long m = m0 + ph * 128 + wm * 64 + b * 16 + frow;
+                    if (m < g.M) store4<TO>(g, m, n, acc[ph][wh][a][b]);
+                }
+        }
+}
+
+// Few rows (a server's single images): bound by the weights' bytes, each read once, straight into the registers of the one
+// wave that multiplies them, so that nothing has to be shared before the end.  A workgroup owns 16 columns; its waves take the
+// k-blocks in turn (neighbouring waves read neighbouring 128 bytes of the same 16 rows), U at a time with the next U on their
+// way, and join their sums through LDS in wave order.  x comes in its own type and the workgroup first quantises what it
+// multiplies into LDS, [block][row][128 bytes] with the exponent bytes behind: no second launch (measured on one row, 4096 x
+// 50176: 43 us, 4.8 TB/s; quantising in the multiplying lanes instead took 77 us, 15 of 16 of them have no row of their own).
+template <typename T, typename TO>
+__global__ void __launch_bounds__(1024) fp8_rows_kernel(GemmArgs g, const T* x, long long ldx, long long K) {
+    constexpr bool EXACT = sizeof(TO) == 4;
+    constexpr int U = 4;
+    __shared__ f32x4 red[16][64];
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int lane = threadIdx.x & 63, frow = lane & 15, fk = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), nw = (int)(blockDim.x >> 6);
+    const long long n0 = (long long)blockIdx.x * 16, ld = (long long)g.kblocks * 128;
+    const int kb0 = (int)blockIdx.y * g.per_split;
+    const int kb1 = kb0 + g.per_split < g.kblocks ? kb0 + g.per_split : g.kblocks;
+    const int rows = (int)g.M, nkb = kb1 - kb0;
+    const long long nrow = n0 + frow < g.N ? n0 + frow : g.N - 1;   // (the last row again: its columns are not stored)
+    const unsigned char* bp = g.b + nrow * ld + fk * 16;
+    const unsigned char* bsp = g.bs + (n0 >> 7) * g.kblocks;
+    const bool live = frow < rows;
+    unsigned char* const sx = smem + (long long)nkb * rows * 128;
+
+    i32x4 b[2][U][2];
+    int sb[2][U];
+    auto fetch = [&](int kb, auto into) {
+        constexpr int I = decltype(into)::value;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = kb + u * nw;
+            if (k >= kb1) break;
+            b[I][u][0] = *reinterpret_cast<const i32x4*>(bp + (long long)k * 128);
+            b[I][u][1] = *reinterpret_cast<const i32x4*>(bp + (long long)k * 128 + 64);
+            sb[I][u] = bsp[k];
+        }
+    };
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](int kb, auto from) {
+        constexpr int I = decltype(from)::value;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = kb + u * nw;
+            if (k >= kb1) break;
+            const i32x4 none = {0, 0, 0, 0};
+            i32x4 lo = none, hi = none;
+            int s = 127;
+            if (live) {
+                const unsigned char* p = smem + ((long long)(k - kb0) * rows + frow) * 128 + fk * 16;
+                lo = *reinterpret_cast<const i32x4*>(p);
+                hi = *reinterpret_cast<const i32x4*>(p + 64);
+                s = sx[(k - kb0) * rows + frow];
+            }
+            const i32x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            const i32x8 w = __builtin_shufflevector(b[I][u][0], b[I][u][1], 0, 1, 2, 3, 4, 5, 6, 7);
+            if constexpr (EXACT) {
+                bf16x8 wa[4], wb[4];
+                widen(v, __uint_as_float((unsigned)s << 23), wa);
+                widen(w, __uint_as_float((unsigned)sb[I][u] << 23), wb);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[q], wa[q], acc, 0, 0, 0);
+            } else acc = mfma_fp8<0, 0>(w, v, acc, sb[I][u], s);
+        }
+    };
+    const std::integral_constant<int, 0> A;
+    const std::integral_constant<int, 1> B;
+    const int step = nw * U;
+    fetch(kb0 + wave, A);
+    {   // while the first weights are on their way: 16 lanes x 8 elements per block, as quant_rows_kernel
+        const int l = threadIdx.x & 15, groups = (int)(blockDim.x >> 4);
+        for (int id = (int)(threadIdx.x >> 4); id < nkb * rows; id += groups) {
+            const int blk = id / rows, m = id - blk * rows;
+            const long long k = (long long)(kb0 + blk) * 128 + l * 8;
+            float v[8], top = 0.0f;
+            load_vec8(x + m * ldx + k, K - k, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(v[j]));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+            const int e = scale_exponent(top);
+            const float f = pow2(-e);
+            *reinterpret_cast<uint2*>(smem + (long long)id * 128 + l * 8) =
+                make_uint2(pack4(v[0] * f, v[1] * f, v[2] * f, v[3] * f), pack4(v[4] * f, v[5] * f, v[6] * f, v[7] * f));
+            if (l == 0) sx[id] = (unsigned char)(e + 127);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        barrier();
+    }
+    for (int kb = kb0 + wave; kb < kb1; kb += 2 * step) {
+        fetch(kb + step, B);
+        multiply(kb, A);
+        fetch(kb + 2 * step, A);
+        multiply(kb + step, B);
+    }
+    red[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0) {
+        for (int w = 1; w < nw; ++w) acc += red[w][lane];
+        const long long n = n0 + fk * 4;
+        if (live && n < g.N) {
+            if (g.splits > 1) store_part(g, blockIdx.y, frow, n, acc);
+            else store4<TO>(g, frow, n, acc);
         }
     }
 }
@@ -372,26 +702,48 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(GemmArgs g) {
     }
 }
 
-struct Plan { int bm, bn, splits, per_split; };
-Plan plan(long long M, long long N, int kblocks) {
-    Plan p;
-    p.bm = M <= 64 ? 64 : 128;
-    p.bn = 128;
-    const long long tiles = yfs_cdiv(M, p.bm) * yfs_cdiv(N, p.bn);
-    long long s = tiles >= 256 ? 1 : 512 / tiles;
-    if (s > kblocks / 2) s = kblocks / 2;
+constexpr int kRows = 16;              // rows that fp8_rows_kernel can take
+constexpr size_t kRowsLds = 128 * 1024;   // its quantised rows in LDS
+constexpr int kCUs = 256;
+
+struct Plan { int kind, bm, bn, splits, per_split; };   // kind 0: fp8_rows_kernel, 1: fp8_gemm_kernel, 2: fp8_gemm8_kernel
+size_t rows_lds(long long M, int per_split) { return ((size_t)per_split * M * 129 + 15) & ~(size_t)15; }
+void set_splits(Plan& p, long long s, int kblocks) {
     if (s < 1) s = 1;
     p.per_split = (int)yfs_cdiv(kblocks, s);
     p.splits = (int)yfs_cdiv(kblocks, p.per_split);
+}
+// Operands that are both in 8 bits.
+Plan plan_tiles(long long M, long long N, int kblocks, bool exact) {
+    Plan p = {1, 128, 128, 1, kblocks};
+    if (!exact && M > 128 && yfs_cdiv(M, 256) * yfs_cdiv(N, 256) >= kCUs && kblocks >= 4) {
+        p.kind = 2;
+        p.bm = p.bn = 256;
+        return p;
+    }
+    if (M <= 64) p.bm = p.bn = 64;
+    const long long tiles = yfs_cdiv(M, p.bm) * yfs_cdiv(N, p.bn);
+    long long s = tiles >= kCUs ? 1 : 2 * kCUs / tiles;
+    if (s > kblocks / 4) s = kblocks / 4;
+    set_splits(p, s, kblocks);
     return p;
 }
+// x in its own type: few enough rows are quantised by the workgroups that multiply them.
+Plan plan_matmul(long long M, long long N, int kblocks, bool exact) {
+    if (M <= kRows) {
+        Plan p = {0, 16, 16, 1, kblocks};
+        const long long tiles = yfs_cdiv(N, 16);
+        long long s = tiles >= kCUs ? 1 : kCUs / tiles;
+        if (s > kblocks / 64) s = kblocks / 64;
+        set_splits(p, s, kblocks);
+        if (rows_lds(M, p.per_split) <= kRowsLds) return p;
+    }
+    return plan_tiles(M, N, kblocks, exact);
+}
+size_t part_bytes(const Plan& p, long long M, long long N) { return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0; }
 
-template <int FM, int FN, int WM, int WN, bool ROWB, bool EXACT, typename TO>
-int launch_tiles(const GemmArgs& g, hipStream_t s) {
-    constexpr int BM = WM * FM * 16, BN = WN * FN * 16;
-    const dim3 grid((unsigned)yfs_cdiv(g.N, BN), (unsigned)yfs_cdiv(g.M, BM), (unsigned)g.splits);
-    fp8_gemm_kernel<FM, FN, WM, WN, ROWB, EXACT, TO><<<grid, 64 * WM * WN, 2 * (BM + BN) * 128, s>>>(g);
-    YFS_CHECK_LAUNCH("fp8_gemm_kernel");
+template <typename TO>
+int join(const GemmArgs& g, hipStream_t s) {
     if (g.splits > 1) {
         long long nb = yfs_cdiv(g.M * ((g.N + 3) / 4), 256);
         fp8_join_kernel<TO><<<dim3((unsigned)(nb < 4096 ? nb : 4096)), 256, 0, s>>>(g);
@@ -400,19 +752,64 @@ int launch_tiles(const GemmArgs& g, hipStream_t s) {
     return YFS_OK;
 }
 
+template <int FM, int FN, int WM, int WN, int S, bool ROWB, bool EXACT, typename TO>
+int launch_tiles(const GemmArgs& g, hipStream_t s) {
+    constexpr int BM = WM * FM * 16, BN = WN * FN * 16, NW = WM * WN;
+    constexpr int STAGE = (BM + BN) * 128 + NW * 256 * (ROWB ? 2 : 1);
+    const dim3 grid((unsigned)yfs_cdiv(g.N, BN), (unsigned)yfs_cdiv(g.M, BM), (unsigned)g.splits);
+    auto kern = fp8_gemm_kernel<FM, FN, WM, WN, S, ROWB, EXACT, TO>;
+    // a short reduction leaves the rest of the ring to other workgroups
+    const int lds = STAGE * (g.per_split < S ? g.per_split : S);
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, STAGE * S);
+    YFS_REQUIRE(e == hipSuccess, YFS_ERR_LAUNCH, "fp8_gemm_kernel: cannot reserve %d bytes of LDS", STAGE * S);
+    kern<<<grid, 64 * NW, lds, s>>>(g);
+    YFS_CHECK_LAUNCH("fp8_gemm_kernel");
+    yfs_note_kernel("fp8_gemm_kernel<%d,%d,splits%d>", BM, BN, g.splits);
+    return join<TO>(g, s);
+}
+
+template <typename TO>
+int launch_gemm8(const GemmArgs& g, hipStream_t s) {
+    auto kern = fp8_gemm8_kernel<TO>;
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, G8_LDS);
+    YFS_REQUIRE(e == hipSuccess, YFS_ERR_LAUNCH, "fp8_gemm8_kernel: cannot reserve %d bytes of LDS", G8_LDS);
+    kern<<<dim3((unsigned)(yfs_cdiv(g.M, 256) * yfs_cdiv(g.N, 256))), 512, G8_LDS, s>>>(g);
+    YFS_CHECK_LAUNCH("fp8_gemm8_kernel");
+    yfs_note_kernel("fp8_gemm8_kernel");
+    return YFS_OK;
+}
+
 template <bool ROWB, bool EXACT, typename TO>
 int gemm(GemmArgs g, hipStream_t s) {
-    const Plan p = plan(g.M, g.N, g.kblocks);
+    const Plan p = plan_tiles(g.M, g.N, g.kblocks, EXACT || ROWB);
     g.splits = p.splits;
     g.per_split = p.per_split;
     g.groups_a = groups64(g.M);
     g.groups_b = groups64(g.N);
-    if (p.bm == 64) return launch_tiles<4, 2, 1, 4, ROWB, EXACT, TO>(g, s);
-    return launch_tiles<4, 4, 2, 2, ROWB, EXACT, TO>(g, s);
+    if constexpr (!EXACT && !ROWB) {
+        if (p.kind == 2) return launch_gemm8<TO>(g, s);
+    }
+    if (p.bm == 64) return launch_tiles<2, 2, 2, 2, 4, ROWB, EXACT, TO>(g, s);
+    return launch_tiles<4, 4, 2, 2, 2, ROWB, EXACT, TO>(g, s);
 }
-size_t part_bytes(long long M, long long N, int kblocks) {
-    const Plan p = plan(M, N, kblocks);
-    return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
+
+template <typename T, typename TO>
+int matmul_rows(GemmArgs g, const Plan& p, const void* x, long long ldx, long long K, hipStream_t s) {
+    g.splits = p.splits;
+    g.per_split = p.per_split;
+    auto kern = fp8_rows_kernel<T, TO>;
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kRowsLds);
+    YFS_REQUIRE(e == hipSuccess, YFS_ERR_LAUNCH, "fp8_rows_kernel: cannot reserve %d bytes of LDS", (int)kRowsLds);
+    const int waves = p.per_split >= 16 ? 16 : (p.per_split >= 8 ? 8 : 4);
+    kern<<<dim3((unsigned)yfs_cdiv(g.N, 16), (unsigned)p.splits), 64 * waves, rows_lds(g.M, p.per_split), s>>>(g, (const T*)x, ldx, K);
+    YFS_CHECK_LAUNCH("fp8_rows_kernel");
+    yfs_note_kernel("fp8_rows_kernel<splits%d>", g.splits);
+    return join<TO>(g, s);
+}
+template <typename T>
+int matmul_rows(const GemmArgs& g, const Plan& p, const void* x, long long ldx, long long K, int out_dtype, hipStream_t s) {
+    if (out_dtype == YFS_F32) return matmul_rows<T, float>(g, p, x, ldx, K, s);
+    return out_dtype == YFS_BF16 ? matmul_rows<T, bf16_t>(g, p, x, ldx, K, s) : matmul_rows<T, _Float16>(g, p, x, ldx, K, s);
 }
 
 bool known(int d) { return d == YFS_F32 || d == YFS_BF16 || d == YFS_F16; }
@@ -455,12 +852,14 @@ YFS_API int yfs_fp8_quantize_rows(const void* x, int dtype, int64_t ld, int64_t 
                          groups64(M), groups64(K)};
     hipStream_t s = (hipStream_t)stream;
     if (q && qt) return quantize<false, true, true>(g, dtype, s);
-    return q ? quantize<false, true, false>(g, dtype, s) : quantize<false, false, true>(g, dtype, s);
+    if (q) return colsum ? quantize<false, true, false>(g, dtype, s) : quantize_rows_only(g, dtype, s);
+    return quantize<false, false, true>(g, dtype, s);
 }
 
+// (whatever the output's type: the larger of the two forms)
 YFS_API size_t yfs_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0 || M > kMost || N > kMost || K > kMost) return 0;
-    return part_bytes(M, N, (int)yfs_cdiv(K, 128));
+    return part_bytes(plan_tiles(M, N, (int)yfs_cdiv(K, 128), true), M, N);
 }
 
 YFS_API int yfs_fp8_gemm(const void* aq, const void* a_scale, const void* bq, const void* b_scale, int b_row_scales, const float* bias,
@@ -490,7 +889,10 @@ YFS_API int yfs_fp8_gemm(const void* aq, const void* a_scale, const void* bq, co
 namespace {
 struct MatmulSpace { size_t q, s, part; };
 MatmulSpace matmul_space(long long M, long long N, long long K) {
-    return {align256((size_t)(M * pad128(K))), align256((size_t)packed_bytes(M, yfs_cdiv(K, 128))), part_bytes(M, N, (int)yfs_cdiv(K, 128))};
+    const int kb = (int)yfs_cdiv(K, 128);
+    const Plan p = plan_matmul(M, N, kb, true);
+    if (p.kind == 0) return {0, 0, part_bytes(p, M, N)};
+    return {align256((size_t)(M * pad128(K))), align256((size_t)packed_bytes(M, kb)), part_bytes(p, M, N)};
 }
 }  // namespace
 
@@ -505,9 +907,22 @@ YFS_API int yfs_fp8_matmul(const void* x, int x_dtype, int64_t ld, const void* w
                            void* stream) {
     YFS_REQUIRE(x && wq && w_scale && y, YFS_ERR_INVALID_ARG, "yfs_fp8_matmul: null pointer");
     REQUIRE_SIZES("yfs_fp8_matmul", M, N, K);
+    YFS_REQUIRE(known(x_dtype) && known(out_dtype), YFS_ERR_UNSUPPORTED, "yfs_fp8_matmul: unknown dtype %d or %d", x_dtype, out_dtype);
+    YFS_REQUIRE(ld >= 0, YFS_ERR_INVALID_ARG, "yfs_fp8_matmul: negative row stride");
+    YFS_REQUIRE(slope >= 0.0f && slope <= 1.0f, YFS_ERR_INVALID_ARG, "yfs_fp8_matmul: slope %g not in [0, 1]", slope);
+    REQUIRE_ALIGNED("yfs_fp8_matmul", wq);
     const size_t need = yfs_fp8_matmul_workspace_bytes(M, N, K);
-    YFS_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0, YFS_ERR_WORKSPACE,
-                "yfs_fp8_matmul: workspace needs %zu bytes, 256-byte aligned", need);
+    YFS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
+                YFS_ERR_WORKSPACE, "yfs_fp8_matmul: workspace needs %zu bytes, 256-byte aligned", need);
+    const Plan p = plan_matmul(M, N, (int)yfs_cdiv(K, 128), true);
+    if (p.kind == 0) {
+        const GemmArgs g = {nullptr, nullptr, (const unsigned char*)wq, (const unsigned char*)w_scale, bias, y, (float*)workspace,
+                            M, N, (int)yfs_cdiv(K, 128), 1, 0, 0, 0, slope, 0};
+        hipStream_t s = (hipStream_t)stream;
+        if (x_dtype == YFS_F32) return matmul_rows<float>(g, p, x, ld, K, out_dtype, s);
+        if (x_dtype == YFS_BF16) return matmul_rows<bf16_t>(g, p, x, ld, K, out_dtype, s);
+        return matmul_rows<_Float16>(g, p, x, ld, K, out_dtype, s);
+    }
     const MatmulSpace w = matmul_space(M, N, K);
     unsigned char* q = (unsigned char*)workspace;
     const int rc = yfs_fp8_quantize_rows(x, x_dtype, ld, M, K, q, q + w.q, nullptr, nullptr, nullptr, stream);
