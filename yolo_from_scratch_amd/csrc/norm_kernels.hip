@@ -129,31 +129,101 @@ struct BwdArgs {
     float *dw, *db;       // results, or partial sums [parts][2][cols]
     long long rows;
     int cols, lg;
+    int dx_blocks;        // workgroups before this index do dx, the others column sums
+    int strips;           // of 32 vectors of columns
+    long long part_rows;  // rows per partial sum
 };
 
-template <typename T, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_dx_kernel(BwdArgs g) {
+// dw, db of a strip of 32 * VE columns over the rows of one part: 32 column threads x (blockDim / 32) row slices, joined in
+// slice order.
+template <typename T>
+__device__ __forceinline__ void column_sums(const BwdArgs& g, int block, float* red) {
+    constexpr int VE = 16 / sizeof(T);
+    const int ct = threadIdx.x & 31, rs = threadIdx.x >> 5, slices = (int)blockDim.x >> 5, wave = threadIdx.x >> 6;
+    const int part = block / g.strips, strip = block - part * g.strips;
+    const long long c = ((long long)strip * 32 + ct) * VE, n = g.cols - c;
+    const long long lo = part * g.part_rows, hi = lo + g.part_rows < g.rows ? lo + g.part_rows : g.rows;
+    float aw[VE], ab[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) aw[j] = ab[j] = 0.0f;
+    if (n > 0) {
+#pragma unroll 4
+        for (long long row = lo + rs; row < hi; row += slices) {
+            const float mu = g.mean[row], r = g.rstd[row];
+            float h[VE], d[VE];
+            load_vec((const T*)g.x + row * g.xs + c, n, h);
+            load_vec((const T*)g.dy + row * g.dys + c, n, d);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                aw[j] += j < n ? d[j] * ((h[j] - mu) * r) : 0.0f;
+                ab[j] += d[j];
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+        aw[j] += __shfl_xor(aw[j], 32, 64);
+        ab[j] += __shfl_xor(ab[j], 32, 64);
+        if ((threadIdx.x & 32) == 0) {
+            red[(wave * 2 + 0) * 32 * VE + ct * VE + j] = aw[j];
+            red[(wave * 2 + 1) * 32 * VE + ct * VE + j] = ab[j];
+        }
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < 2 * 32 * VE; k += blockDim.x) {
+        const int which = k / (32 * VE), cc = k % (32 * VE);
+        const long long col = (long long)strip * 32 * VE + cc;
+        if (col >= g.cols) continue;
+        float s = 0.0f;
+        for (int q = 0; q < slices / 2; ++q) s += red[(q * 2 + which) * 32 * VE + cc];
+        float* out = which ? g.db : g.dw;
+        if (out) out[(long long)part * 2 * g.cols + col] = s;
+    }
+}
+
+// dx by rows as in the forward pass.  ACC: the thread that holds a column of dx sums its dw and db too, over the rows that its
+// workgroup meets: x and dy are read once for all three.  That needs many rows per workgroup, or the partial sums outgrow them
+// (200704 x 256 bf16: 53 + 114 us as two kernels); for few rows the column sums are other workgroups of the same launch.
+template <typename T, int NV, bool BLOCK, bool ACC>
+__global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_bwd_kernel(BwdArgs g) {
     constexpr int VE = 16 / sizeof(T);
     __shared__ float2 red[32];
+    extern __shared__ float sums[];
+    if (!ACC && (int)blockIdx.x >= g.dx_blocks) {
+        column_sums<T>(g, (int)blockIdx.x - g.dx_blocks, sums);
+        return;
+    }
     const int G = BLOCK ? (int)blockDim.x : 1 << g.lg;
     const int t = BLOCK ? (int)threadIdx.x : (int)threadIdx.x & (G - 1);
     const long long rpb = BLOCK ? 1 : 256 >> g.lg;
     const float inv = 1.0f / (float)g.cols;
+    float wv[NV][VE], aw[ACC ? NV : 1][VE], ab[ACC ? NV : 1][VE];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * G + t) * VE;
+        load_vec_or(g.w, c, g.cols - c, wv[i], 1.0f);
+        if (ACC) {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) aw[i][j] = ab[i][j] = 0.0f;
+        }
+    }
     int slot = 0;
-    for (long long row = (long long)blockIdx.x * rpb + (BLOCK ? 0 : (int)threadIdx.x >> g.lg); row < g.rows; row += (long long)gridDim.x * rpb) {
+    for (long long row = (long long)blockIdx.x * rpb + (BLOCK ? 0 : (int)threadIdx.x >> g.lg); row < g.rows; row += (long long)g.dx_blocks * rpb) {
         const float mu = g.mean[row], r = g.rstd[row];
         float h[NV][VE], d[NV][VE], s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * G + t) * VE, n = g.cols - c;
-            float wv[VE];
             load_vec((const T*)g.x + row * g.xs + c, n, h[i]);
             load_vec((const T*)g.dy + row * g.dys + c, n, d[i]);
-            load_vec_or(g.w, c, n, wv, 1.0f);
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
                 h[i][j] = j < n ? (h[i][j] - mu) * r : 0.0f;
-                d[i][j] *= wv[j];
+                if (ACC) {
+                    aw[i][j] += d[i][j] * h[i][j];
+                    ab[i][j] += d[i][j];
+                }
+                d[i][j] *= wv[i][j];
                 s1 += d[i][j];
                 s2 += d[i][j] * h[i][j];
             }
@@ -169,15 +239,44 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_dx_kernel(BwdArgs g) {
             store_vec((T*)g.dx + row * g.cols + c, g.cols - c, d[i]);
         }
     }
+    if constexpr (ACC && BLOCK) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * G + t) * VE;
+            store_vec(g.dw + (long long)blockIdx.x * 2 * g.cols + c, g.cols - c, aw[i]);
+            store_vec(g.db + (long long)blockIdx.x * 2 * g.cols + c, g.cols - c, ab[i]);
+        }
+    } else if constexpr (ACC) {
+        const int grp = (int)threadIdx.x >> g.lg, groups = 256 >> g.lg, width = G * NV * VE;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                sums[(grp * 2 + 0) * width + (i * G + t) * VE + j] = aw[i][j];
+                sums[(grp * 2 + 1) * width + (i * G + t) * VE + j] = ab[i][j];
+            }
+        __syncthreads();
+        for (int k = threadIdx.x; k < 2 * g.cols; k += 256) {
+            const int which = k >= g.cols, c = k - which * g.cols;
+            float v = 0.0f;
+            for (int q = 0; q < groups; ++q) v += sums[(q * 2 + which) * width + c];
+            g.dw[(long long)blockIdx.x * 2 * g.cols + k] = v;   // (db lies cols behind dw)
+        }
+    }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(1024) ln_dx_long_kernel(BwdArgs g) {
+__global__ void __launch_bounds__(1024) ln_bwd_long_kernel(BwdArgs g) {
     constexpr int VE = 16 / sizeof(T);
     __shared__ float2 red[32];
+    extern __shared__ float sums[];
+    if ((int)blockIdx.x >= g.dx_blocks) {
+        column_sums<T>(g, (int)blockIdx.x - g.dx_blocks, sums);
+        return;
+    }
     const float inv = 1.0f / (float)g.cols;
     int slot = 0;
-    for (long long row = blockIdx.x; row < g.rows; row += gridDim.x) {
+    for (long long row = blockIdx.x; row < g.rows; row += g.dx_blocks) {
         const T *xr = (const T*)g.x + row * g.xs, *dr = (const T*)g.dy + row * g.dys;
         const float mu = g.mean[row], r = g.rstd[row];
         float h[VE], d[VE], wv[VE], s1 = 0.0f, s2 = 0.0f;
@@ -207,77 +306,25 @@ __global__ void __launch_bounds__(1024) ln_dx_long_kernel(BwdArgs g) {
     }
 }
 
-// dw, db of a strip of 32 * VE columns over the rows of one part: 32 column threads x 8 row slices, joined in slice order.
-template <typename T>
-__global__ void __launch_bounds__(256) ln_dwdb_kernel(BwdArgs g, long long rows_per_part) {
-    constexpr int VE = 16 / sizeof(T);
-    __shared__ float red[8][2][32 * VE + 4];
-    const int ct = threadIdx.x & 31, rs = threadIdx.x >> 5;
-    const long long c = ((long long)blockIdx.x * 32 + ct) * VE, n = g.cols - c;
-    const long long lo = (long long)blockIdx.y * rows_per_part;
-    const long long hi = lo + rows_per_part < g.rows ? lo + rows_per_part : g.rows;
-    float aw[VE], ab[VE];
-#pragma unroll
-    for (int j = 0; j < VE; ++j) aw[j] = ab[j] = 0.0f;
-    if (n > 0) {
-        for (long long row = lo + rs; row < hi; row += 8) {
-            const float mu = g.mean[row], r = g.rstd[row];
-            float h[VE], d[VE];
-            load_vec((const T*)g.x + row * g.xs + c, n, h);
-            load_vec((const T*)g.dy + row * g.dys + c, n, d);
-#pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                aw[j] += j < n ? d[j] * ((h[j] - mu) * r) : 0.0f;
-                ab[j] += d[j];
-            }
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < VE; ++j) {
-        red[rs][0][ct * VE + j] = aw[j];
-        red[rs][1][ct * VE + j] = ab[j];
-    }
-    __syncthreads();
-    for (int k = threadIdx.x; k < 2 * 32 * VE; k += 256) {
-        const int which = k / (32 * VE), cc = k % (32 * VE);
-        const long long col = (long long)blockIdx.x * 32 * VE + cc;
-        if (col >= g.cols) continue;
-        float s = 0.0f;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) s += red[q][which][cc];
-        float* out = which ? g.db : g.dw;
-        if (out) out[(long long)blockIdx.y * 2 * g.cols + col] = s;
-    }
-}
-
-// dw, db from partial sums [parts][2][cols], in the order of the parts
-__global__ void __launch_bounds__(256) ln_reduce_kernel(const float* __restrict__ part, int parts, int cols, float* __restrict__ dw,
-                                                        float* __restrict__ db) {
-    __shared__ float red[8][32];
+// dw, db from partial sums [parts][2][cols]: 32 columns x 32 slices of the parts, joined in slice order
+__global__ void __launch_bounds__(1024) ln_reduce_kernel(const float* __restrict__ part, int parts, int cols, float* __restrict__ dw,
+                                                         float* __restrict__ db) {
+    __shared__ float red[32][33];
     const int ct = threadIdx.x & 31, ps = threadIdx.x >> 5;
     const long long k = (long long)blockIdx.x * 32 + ct;   // column of [2][cols]
     float s = 0.0f;
-    if (k < 2LL * cols)
-        for (int p = ps; p < parts; p += 8) s += part[(long long)p * 2 * cols + k];
+    if (k < 2LL * cols) {
+#pragma unroll 8
+        for (int p = ps; p < parts; p += 32) s += part[(long long)p * 2 * cols + k];
+    }
     red[ps][ct] = s;
     __syncthreads();
     if (ps == 0 && k < 2LL * cols) {
 #pragma unroll
-        for (int q = 1; q < 8; ++q) s += red[q][ct];
+        for (int q = 1; q < 32; ++q) s += red[q][ct];
         float* out = k < cols ? dw : db;
         if (out) out[k < cols ? k : k - cols] = s;
     }
-}
-
-constexpr int kMaxParts = 256;
-// Rows are summed by one workgroup per strip as long as they are few; the rest goes over up to kMaxParts parts.
-int dwdb_parts(long long rows, int cols, int esize) {
-    const long long strips = yfs_cdiv(cols, 32 * (16 / esize));
-    long long parts = yfs_cdiv(2048, strips);
-    const long long most = yfs_cdiv(rows, 64);
-    if (parts > most) parts = most;
-    if (parts > kMaxParts) parts = kMaxParts;
-    return (int)(parts < 1 ? 1 : parts);
 }
 
 struct Shape { int nv, lg, threads; };   // threads > 256 or lg < 0: one workgroup per row; nv == 0: the long form
@@ -295,6 +342,34 @@ Shape ln_shape(int cols, int esize, int max_nv_block) {
 unsigned row_blocks(long long rows, const Shape& s) {
     const long long nb = s.lg >= 0 ? yfs_cdiv(rows, 256 >> s.lg) : rows;
     return (unsigned)(nb < 8192 ? nb : 8192);
+}
+
+// How the backward pass goes over the chip.  acc: dx and the column sums by the same workgroups, one partial sum each; else
+// column sums by workgroups of their own, over `parts` parts of the rows.
+struct BwdPlan { Shape sh; bool acc; int dx_blocks, strips, parts; long long part_rows; };
+BwdPlan bwd_plan(long long rows, int cols, int esize, bool need_dx) {
+    BwdPlan p;
+    p.sh = ln_shape(cols, esize, esize == 2 ? 2 : 4);
+    p.dx_blocks = need_dx ? (int)row_blocks(rows, p.sh) : 0;
+    p.strips = (int)yfs_cdiv(cols, 32 * (16 / esize));
+    const long long rpb = p.sh.lg >= 0 ? 256 >> p.sh.lg : 1;
+    // a partial sum is 8 bytes a column, a row of x, dy and dx 6 or 12: from 8 rows a workgroup on it is small next to them
+    const long long fill = p.sh.threads == 256 ? 1024 : (p.sh.threads == 512 ? 512 : 256);
+    p.acc = need_dx && p.sh.nv > 0 && p.sh.nv <= 2 && rows >= fill / 2 * rpb * 8;
+    if (p.acc) {
+        const long long nb = rows / (rpb * 8);
+        p.dx_blocks = (int)(nb < fill ? nb : fill);
+        p.parts = p.dx_blocks;
+        p.part_rows = 0;
+        return p;
+    }
+    const long long slices = p.sh.threads / 32;
+    long long parts = yfs_cdiv(2048, p.strips), most = yfs_cdiv(rows, slices * 16);
+    if (parts > most) parts = most;
+    if (parts > 256) parts = 256;
+    p.part_rows = yfs_cdiv(rows, parts);
+    p.parts = (int)yfs_cdiv(rows, p.part_rows);
+    return p;
 }
 
 template <typename T>
@@ -321,38 +396,43 @@ int fwd(const void* x, long long xs, const float* w, const float* b, void* y, fl
 
 template <typename T>
 int bwd(BwdArgs g, float* part, hipStream_t s) {
-    if (g.dx) {
-        const Shape sh = ln_shape(g.cols, sizeof(T), sizeof(T) == 2 ? 2 : 4);
-        g.lg = sh.lg;
-        const dim3 grid(row_blocks(g.rows, sh)), blk(sh.threads);
-        if (sh.nv == 0) ln_dx_long_kernel<T><<<grid, blk, 0, s>>>(g);
-        else if (sh.lg >= 0) {
-            if (sh.nv == 1) ln_dx_kernel<T, 1, false><<<grid, blk, 0, s>>>(g);
-            else ln_dx_kernel<T, 2, false><<<grid, blk, 0, s>>>(g);
-        } else switch (sh.nv) {
-            case 1: ln_dx_kernel<T, 1, true><<<grid, blk, 0, s>>>(g); break;
-            case 2: ln_dx_kernel<T, 2, true><<<grid, blk, 0, s>>>(g); break;
-            default:
-                if constexpr (sizeof(T) == 4) ln_dx_kernel<T, 4, true><<<grid, blk, 0, s>>>(g);
-        }
-        YFS_CHECK_LAUNCH("ln_dx_kernel");
+    const bool sums = g.dw || g.db;
+    BwdPlan p = bwd_plan(g.rows, g.cols, sizeof(T), g.dx != nullptr);
+    if (!sums) {
+        p.acc = false;
+        p.parts = 0;
+        p.dx_blocks = (int)row_blocks(g.rows, p.sh);
     }
-    if (g.dw || g.db) {
-        const int parts = dwdb_parts(g.rows, g.cols, sizeof(T));
-        const long long per = yfs_cdiv(g.rows, parts);
-        const dim3 grid((unsigned)yfs_cdiv(g.cols, 32 * (16 / sizeof(T))), (unsigned)parts);
-        if (parts == 1) {
-            ln_dwdb_kernel<T><<<grid, 256, 0, s>>>(g, per);
-            YFS_CHECK_LAUNCH("ln_dwdb_kernel");
-        } else {
-            float *dw = g.dw, *db = g.db;
-            g.dw = part;
-            g.db = part + g.cols;
-            ln_dwdb_kernel<T><<<grid, 256, 0, s>>>(g, per);
-            YFS_CHECK_LAUNCH("ln_dwdb_kernel");
-            ln_reduce_kernel<<<dim3((unsigned)yfs_cdiv(2LL * g.cols, 32)), 256, 0, s>>>(part, parts, g.cols, dw, db);
-            YFS_CHECK_LAUNCH("ln_reduce_kernel");
-        }
+    g.lg = p.sh.lg;
+    g.dx_blocks = p.dx_blocks;
+    g.strips = p.strips;
+    g.part_rows = p.part_rows;
+    float *dw = g.dw, *db = g.db;
+    const bool join = p.acc || p.parts > 1;
+    if (join) {
+        g.dw = part;
+        g.db = part + g.cols;
+    }
+    if (!sums && !g.dx) return YFS_OK;
+    const dim3 grid((unsigned)(p.dx_blocks + (p.acc ? 0 : (long long)p.strips * p.parts))), blk(p.sh.threads);
+    // sums of the groups of a workgroup, or of the waves of a column strip
+    const size_t lds = p.acc ? (p.sh.lg >= 0 ? 512 * sizeof(float) * p.sh.nv * (16 / sizeof(T)) : 0)
+                             : (sums ? (size_t)p.sh.threads / 64 * 2 * 32 * (16 / sizeof(T)) * sizeof(float) : 0);
+#define LN_BWD(NV, BLOCK) \
+    do { if (p.acc) ln_bwd_kernel<T, NV, BLOCK, true><<<grid, blk, lds, s>>>(g); else ln_bwd_kernel<T, NV, BLOCK, false><<<grid, blk, lds, s>>>(g); } while (0)
+    if (p.sh.nv == 0) ln_bwd_long_kernel<T><<<grid, blk, lds, s>>>(g);
+    else if (p.sh.lg >= 0) {
+        if (p.sh.nv == 1) LN_BWD(1, false); else LN_BWD(2, false);
+    } else if (p.sh.nv == 1) LN_BWD(1, true);
+    else if (p.sh.nv == 2) LN_BWD(2, true);
+    else {
+        if constexpr (sizeof(T) == 4) ln_bwd_kernel<T, 4, true, false><<<grid, blk, lds, s>>>(g);
+    }
+#undef LN_BWD
+    YFS_CHECK_LAUNCH("ln_bwd_kernel");
+    if (sums && join) {
+        ln_reduce_kernel<<<dim3((unsigned)yfs_cdiv(2LL * g.cols, 32)), 1024, 0, s>>>(part, p.parts, g.cols, dw, db);
+        YFS_CHECK_LAUNCH("ln_reduce_kernel");
     }
     return YFS_OK;
 }
@@ -374,10 +454,16 @@ YFS_API int yfs_layer_norm_fwd(const void* x, int64_t x_stride, const float* w, 
     return fwd<_Float16>(x, x_stride, w, b, y, mean, rstd, rows, (int)cols, eps, s);
 }
 
+// (with or without dx: the larger of the two)
 YFS_API size_t yfs_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols, int dtype) {
     if (rows <= 0 || cols <= 0 || cols >= (1LL << 30) || !known(dtype)) return 0;
-    const int parts = dwdb_parts(rows, (int)cols, dtype == YFS_F32 ? 4 : 2);
-    return parts == 1 ? 0 : (size_t)parts * 2 * (size_t)cols * sizeof(float);
+    size_t most = 0;
+    for (int dx = 0; dx < 2; ++dx) {
+        const BwdPlan p = bwd_plan(rows, (int)cols, dtype == YFS_F32 ? 4 : 2, dx);
+        const size_t need = p.acc || p.parts > 1 ? (size_t)p.parts * 2 * (size_t)cols * sizeof(float) : 0;
+        most = need > most ? need : most;
+    }
+    return most;
 }
 
 YFS_API int yfs_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* w, const float* mean,
@@ -391,7 +477,7 @@ YFS_API int yfs_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x,
     const size_t need = (dw || db) ? yfs_layer_norm_bwd_workspace_bytes(rows, cols, dtype) : 0;
     YFS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), YFS_ERR_WORKSPACE,
                 "yfs_layer_norm_bwd: workspace needs %zu bytes", need);
-    const BwdArgs g = {dy, x, dy_stride, x_stride, w, mean, rstd, dx, dw, db, rows, (int)cols, 0};
+    const BwdArgs g = {dy, x, dy_stride, x_stride, w, mean, rstd, dx, dw, db, rows, (int)cols, 0, 0, 0, 0};
     hipStream_t s = (hipStream_t)stream;
     if (dtype == YFS_F32) return bwd<float>(g, (float*)workspace, s);
     if (dtype == YFS_BF16) return bwd<__bf16>(g, (float*)workspace, s);
