@@ -116,9 +116,9 @@ def test_refusals_of_the_library():
     assert lib.yfs_fp8_gemm(p, p, p, p, 0, None, p, 1, 8, 8, 8, 3.0, 0, None, 0, None) == -1
     need = lib.yfs_fp8_gemm_workspace_bytes(64, 4096, 50176)
     assert need > 0 and lib.yfs_fp8_gemm(p, p, p, p, 0, None, p, 1, 64, 4096, 50176, 1.0, 0, p, need - 1, None) == -3
-    need = lib.yfs_fp8_matmul_workspace_bytes(3, 40, 200)
-    assert need > 0 and lib.yfs_fp8_matmul(p, 1, 200, p, p, None, p, 1, 3, 40, 200, 1.0, p, need - 1, None) == -3
-    assert lib.yfs_fp8_matmul(p, 1, 200, p, p, None, p, 1, 3, 40, 200, 1.0, p + 16, need, None) == -3
+    need = lib.yfs_fp8_matmul_workspace_bytes(30, 40, 200)
+    assert need > 0 and lib.yfs_fp8_matmul(p, 1, 200, p, p, None, p, 1, 30, 40, 200, 1.0, p, need - 1, None) == -3
+    assert lib.yfs_fp8_matmul(p, 1, 200, p, p, None, p, 1, 30, 40, 200, 1.0, p + 16, need, None) == -3
     assert lib.yfs_fp8_matmul_workspace_bytes(0, 1, 1) == 0 and lib.yfs_fp8_gemm_workspace_bytes(1, big, 1) == 0
     assert lib.yfs_fp8_colsum(p, 0, 8, p, 0, None) == -1
 

@@ -317,3 +317,13 @@ def test_module_matches_torch_names_and_trains():
 def test_library_is_loaded_by_name():
     import yolo_from_scratch_amd as y
     assert hasattr(ctypes.CDLL(y.LIB_PATH), "yfs_layer_norm_bwd")
+
+
+@pytest.mark.gpu
+def test_second_derivative_is_refused():
+    import yolo_from_scratch_amd as yfs
+    x = torch.randn(4, 32, device=DEV, requires_grad=True)
+    for f in (lambda: yfs.layer_norm(x), lambda: yfs.dropout(x, 0.5, 1), lambda: yfs.fp8_linear(x, torch.ones(8, 32, device=DEV))):
+        with pytest.raises(RuntimeError):
+            g, = torch.autograd.grad(f().sum(), x, create_graph=True)
+            g.sum().backward()

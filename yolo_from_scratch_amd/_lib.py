@@ -66,6 +66,26 @@ def _declare(handle):
 KNOBS = {"igemm_tile": 0, "wgrad_tile": 1, "wgrad_splits": 2, "nms_fused": 3, "stem_kernel": 4, "igemm_persist": 5}     # include/yfs.h: yfs_knob_id
 
 
+_binding = None
+
+
+def binding():
+    """The extension module with the tensor side of the head operators (csrc/torch_binding.cpp), given the addresses of the
+    entry points of the library that is loaded (LIB_PATH)."""
+    global _binding
+    if _binding is None:
+        try:
+            from . import _binding as module
+        except ImportError as e:
+            raise YfsError(f"yolo_from_scratch_amd/_binding.so cannot be loaded ({e}): build it with "
+                           f"`make -C {os.path.join(_HERE, 'csrc')}`. There is no CPU fallback.") from e
+        names = ("yfs_last_error", "yfs_layer_norm_fwd", "yfs_layer_norm_bwd", "yfs_layer_norm_bwd_workspace_bytes",
+                 "yfs_dropout_fwd", "yfs_dropout_bwd", "yfs_fp8_matmul", "yfs_fp8_matmul_workspace_bytes")
+        module.init({n: ctypes.cast(getattr(lib(), n), ctypes.c_void_p).value for n in names}, YfsError)
+        _binding = module
+    return _binding
+
+
 def set_knob(name, value):
     """Measurement aid (include/yfs.h, tuning knobs): force a kernel variant; 0 restores the library's own choice."""
     check(lib().yfs_set_knob(ctypes.c_int(KNOBS[name]), ctypes.c_int(int(value))), "yfs_set_knob")

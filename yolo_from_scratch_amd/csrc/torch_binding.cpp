@@ -1,0 +1,272 @@
+// Tensor side of the head operators whose calls are short: layer norm, dropout, the served 8-bit product.  Argument checks,
+// output allocation and the autograd nodes run here instead of in Python, whose interpreter time was several times the
+// kernels' (forward and backward of a layer norm of 64 x 4096: 121 us, 12 of them on the GPU).  The kernels are reached through
+// the addresses of the C ABI's entry points (include/yfs.h) that the Python side hands over from the library it has loaded.
+#include <torch/extension.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <optional>
+#include <stdexcept>
+#include <string>
+
+#include "../../include/yfs.h"
+
+namespace {
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+struct YfsException : std::runtime_error {
+    using std::runtime_error::runtime_error;
+};
+PyObject* g_error = nullptr;
+
+struct Entries {
+    decltype(&yfs_last_error) last_error;
+    decltype(&yfs_layer_norm_fwd) ln_fwd;
+    decltype(&yfs_layer_norm_bwd) ln_bwd;
+    decltype(&yfs_layer_norm_bwd_workspace_bytes) ln_ws;
+    decltype(&yfs_dropout_fwd) drop_fwd;
+    decltype(&yfs_dropout_bwd) drop_bwd;
+    decltype(&yfs_fp8_matmul) matmul;
+    decltype(&yfs_fp8_matmul_workspace_bytes) matmul_ws;
+} yfs;
+
+[[noreturn]] void fail(const std::string& what) { throw YfsException(what); }
+std::string str(const Tensor& t) { return c10::str(t.scalar_type(), " ", t.sizes()); }
+void check(int status, const char* what) {
+    if (status == YFS_OK) return;
+    char buf[512];
+    yfs.last_error(buf, sizeof(buf));
+    fail(c10::str(what, " failed with status ", status, ": ", buf));
+}
+int code(at::ScalarType t) {
+    return t == at::kFloat ? YFS_F32 : (t == at::kBFloat16 ? YFS_BF16 : (t == at::kHalf ? YFS_F16 : -1));
+}
+// all on one GPU
+void on_one_gpu(const char* what, std::initializer_list<const Tensor*> ts) {
+    const Tensor* first = nullptr;
+    for (const Tensor* t : ts) {
+        if (!t || !t->defined()) continue;
+        if (!t->is_cuda())
+            fail("yolo_from_scratch_amd ops run on the MI355X only: got a CPU tensor (there is no CPU fallback; the CPU oracle "
+                 "lives in oracle/ and is test-only)");
+        if (first && t->device() != first->device()) fail(c10::str(what, ": tensors on devices ", first->device(), " and ", t->device()));
+        if (!first) first = t;
+    }
+}
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+float* f32(const Tensor& t) { return t.defined() ? t.mutable_data_ptr<float>() : nullptr; }
+Tensor get(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+
+// a tensor as rows of its last axis, unit stride inside a row
+struct Rows {
+    Tensor t;
+    int64_t rows, cols, stride;
+    explicit Rows(const Tensor& x) : t(x), cols(x.size(-1)) {
+        if (x.dim() == 2 && (cols == 1 || x.stride(1) == 1)) {
+            rows = x.size(0);
+            stride = x.stride(0);
+        } else {
+            t = x.contiguous();
+            rows = t.numel() / cols;
+            stride = cols;
+        }
+    }
+};
+Tensor f32_vector(const Tensor& t) {
+    return t.defined() ? (t.scalar_type() == at::kFloat ? t : t.to(at::kFloat)).contiguous() : t;
+}
+void once(const char* what) {
+    if (at::GradMode::is_enabled()) fail(c10::str(what, ": the gradient is not differentiable (create_graph=True)"));
+}
+
+// ---- layer norm ------------------------------------------------------------------------------------------------------
+Tensor ln_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, Tensor* stats) {
+    const Rows r(x);
+    const Tensor w = f32_vector(weight), b = f32_vector(bias);
+    const c10::DeviceGuard guard(x.device());
+    Tensor y = at::empty(x.sizes(), x.options());
+    if (stats) *stats = at::empty({2, r.rows}, x.options().dtype(at::kFloat));
+    if (r.rows) {
+        float* mean = stats ? f32(*stats) : nullptr;
+        check(yfs.ln_fwd(ptr(r.t), r.stride, f32(w), f32(b), y.mutable_data_ptr(), mean, mean ? mean + r.rows : nullptr, r.rows, r.cols,
+                         (float)eps, code(x.scalar_type()), stream_of(x)),
+              "yfs_layer_norm_fwd");
+    }
+    return y;
+}
+
+struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight_, const OptTensor& bias_, double eps) {
+        const Tensor weight = get(weight_), bias = get(bias_);
+        Tensor stats;
+        Tensor y = ln_forward(x, weight, bias, eps, &stats);
+        ctx->save_for_backward({x, weight, stats});
+        ctx->saved_data["bias"] = bias.defined() ? (int64_t)bias.scalar_type() : -1;
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("layer_norm");
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
+        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+        const bool need_x = ctx->needs_input_grad(0);
+        // (the inputs that are there are counted through)
+        const int64_t bias_type = ctx->saved_data["bias"].toInt();
+        const bool need_w = weight.defined() && ctx->needs_input_grad(1);
+        const bool need_b = bias_type >= 0 && ctx->needs_input_grad(weight.defined() ? 2 : 1);
+        const Rows r(x), d(grads[0].scalar_type() == x.scalar_type() ? grads[0] : grads[0].to(x.scalar_type()));
+        const Tensor w = f32_vector(weight);
+        const c10::DeviceGuard guard(x.device());
+        const auto f = x.options().dtype(at::kFloat);
+        Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : Tensor();
+        Tensor dw = need_w ? (r.rows ? at::empty({r.cols}, f) : at::zeros({r.cols}, f)) : Tensor();
+        Tensor db = need_b ? (r.rows ? at::empty({r.cols}, f) : at::zeros({r.cols}, f)) : Tensor();
+        if (r.rows) {
+            const int type = code(x.scalar_type());
+            const size_t bytes = need_w || need_b ? yfs.ln_ws(r.rows, r.cols, type) : 0;
+            Tensor ws = bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : Tensor();
+            check(yfs.ln_bwd(ptr(d.t), d.stride, ptr(r.t), r.stride, f32(w), f32(stats), f32(stats) + r.rows,
+                             dx.defined() ? dx.mutable_data_ptr() : nullptr, f32(dw), f32(db), r.rows, r.cols, type,
+                             bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(x)),
+                  "yfs_layer_norm_bwd");
+        }
+        if (need_w && weight.scalar_type() != at::kFloat) dw = dw.to(weight.scalar_type());
+        if (need_b && bias_type != (int64_t)at::kFloat) db = db.to((at::ScalarType)bias_type);
+        return {dx, dw, db, Tensor()};
+    }
+};
+
+Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+    if (code(x.scalar_type()) < 0) fail(c10::str("layer_norm: x must be fp32, bf16 or fp16, got ", x.scalar_type()));
+    if (x.dim() == 0 || x.size(-1) == 0) fail(c10::str("layer_norm: x needs a last axis of at least one element, got ", x.sizes()));
+    if (!(eps >= 0)) fail(c10::str("layer_norm: eps must not be negative, got ", eps));
+    const Tensor w = get(weight), b = get(bias);
+    for (const auto& [name, t] : {std::pair<const char*, const Tensor&>("weight", w), std::pair<const char*, const Tensor&>("bias", b)})
+        if (t.defined() && (t.dim() != 1 || t.size(0) != x.size(-1) || !t.is_floating_point()))
+            fail(c10::str("layer_norm: ", name, " must be floating point [", x.size(-1), "], got ", str(t)));
+    on_one_gpu("layer_norm", {&x, &w, &b});
+    if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())))
+        return LayerNormFn::apply(x, weight, bias, eps);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return ln_forward(x, w, b, eps, nullptr);
+}
+
+// ---- dropout ---------------------------------------------------------------------------------------------------------
+Tensor drop(bool backward, const Tensor& in, const Tensor& y, double p, double slope, int64_t seed, const Tensor& seed_dev) {
+    const c10::DeviceGuard guard(in.device());
+    Tensor out = at::empty(in.sizes(), in.options());
+    if (in.numel() == 0) return out;
+    const int64_t* where = seed_dev.defined() ? seed_dev.const_data_ptr<int64_t>() : nullptr;
+    const int type = code(in.scalar_type());
+    if (backward)
+        check(yfs.drop_bwd(ptr(in), ptr(y), out.mutable_data_ptr(), in.numel(), (float)p, (float)slope, (uint64_t)seed, where, type, stream_of(in)),
+              "yfs_dropout_bwd");
+    else
+        check(yfs.drop_fwd(ptr(in), out.mutable_data_ptr(), in.numel(), (float)p, (float)slope, (uint64_t)seed, where, type, stream_of(in)),
+              "yfs_dropout_fwd");
+    return out;
+}
+
+struct DropoutFn : torch::autograd::Function<DropoutFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, double slope, int64_t seed, const OptTensor& seed_) {
+        const Tensor seed_dev = get(seed_);
+        Tensor y = drop(false, x.contiguous(), Tensor(), p, slope, seed, seed_dev);
+        // y is kept for the sign of its elements, a seed in device memory so that a change before backward is noticed
+        ctx->save_for_backward({slope != 1.0 ? y : Tensor(), seed_dev});
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["slope"] = slope;
+        ctx->saved_data["seed"] = seed;
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("dropout");
+        const variable_list saved = ctx->get_saved_variables();
+        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        Tensor dx = drop(true, grads[0].contiguous(), saved[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["slope"].toDouble(),
+                         ctx->saved_data["seed"].toInt(), saved[1]);
+        return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor dropout(const Tensor& x, double p, const py::object& seed, double slope) {
+    if (code(x.scalar_type()) < 0) fail(c10::str("dropout: x must be fp32, bf16 or fp16, got ", x.scalar_type()));
+    if (!(p >= 0.0 && p <= 1.0)) fail(c10::str("dropout: p must lie in [0, 1], got ", p));
+    if (!(slope >= 0.0 && slope <= 1.0)) fail(c10::str("dropout: slope must lie in [0, 1], got ", slope));
+    Tensor dev;
+    int64_t value = 0;
+    if (THPVariable_Check(seed.ptr())) {
+        dev = THPVariable_Unpack(seed.ptr());
+        if (dev.scalar_type() != at::kLong || dev.numel() != 1) fail(c10::str("dropout: a seed tensor must hold one int64, got ", str(dev)));
+    } else if (PyLong_Check(seed.ptr())) {
+        value = (int64_t)PyLong_AsUnsignedLongLongMask(seed.ptr());
+    } else fail(c10::str("dropout: seed must be an int or an int64 tensor, got ", Py_TYPE(seed.ptr())->tp_name));
+    on_one_gpu("dropout", {&x, &dev});
+    if (at::GradMode::is_enabled() && x.requires_grad()) return DropoutFn::apply(x, p, slope, value, dev.defined() ? OptTensor(dev) : std::nullopt);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return drop(false, x.contiguous(), Tensor(), p, slope, value, dev);
+}
+
+// ---- served 8-bit product --------------------------------------------------------------------------------------------
+Tensor fp8_matmul(const Tensor& x, const Tensor& data, const Tensor& scale, int64_t k, const OptTensor& bias, std::optional<double> slope_,
+                  const std::optional<at::ScalarType>& out_dtype) {
+    if (x.dim() == 0 || x.size(-1) != k) fail(c10::str("fp8_matmul: x [..., ", k, "] expected, got ", x.sizes()));
+    if (code(x.scalar_type()) < 0) fail(c10::str("fp8_matmul: x must be fp32, bf16 or fp16, got ", x.scalar_type()));
+    const at::ScalarType out = out_dtype.value_or(x.scalar_type());
+    if (code(out) < 0) fail(c10::str("fp8_matmul: out_dtype must be fp32, bf16 or fp16, got ", out));
+    const double slope = slope_.value_or(1.0);
+    if (!(slope >= 0.0 && slope <= 1.0)) fail(c10::str("fp8_matmul: slope must lie in [0, 1], got ", slope));
+    const int64_t n = data.size(0);
+    const Tensor b = get(bias);
+    if (b.defined() && (b.dim() != 1 || b.size(0) != n || !b.is_floating_point()))
+        fail(c10::str("fp8_matmul: bias must be floating point [", n, "], got ", str(b)));
+    on_one_gpu("fp8_matmul", {&x, &data, &scale, &b});
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Rows r(x);
+    const Tensor bf = f32_vector(b);
+    const c10::DeviceGuard guard(x.device());
+    at::DimVector sizes(x.sizes());
+    sizes.back() = n;
+    Tensor y = at::empty(sizes, x.options().dtype(out));
+    if (r.rows == 0) return y;
+    const size_t bytes = yfs.matmul_ws(r.rows, n, k);
+    Tensor ws = bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : Tensor();
+    check(yfs.matmul(ptr(r.t), code(x.scalar_type()), r.stride, ptr(data), ptr(scale), f32(bf), y.mutable_data_ptr(), code(out), r.rows, n, k,
+                     (float)slope, bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(x)),
+          "yfs_fp8_matmul");
+    return y;
+}
+
+template <typename F>
+void take(F& f, const py::dict& at, const char* name) { f = reinterpret_cast<F>(at[name].cast<uintptr_t>()); }
+
+// addresses: name of each entry point -> its address; error: the exception that refusals raise
+void init(const py::dict& addresses, const py::object& error) {
+    take(yfs.last_error, addresses, "yfs_last_error");
+    take(yfs.ln_fwd, addresses, "yfs_layer_norm_fwd");
+    take(yfs.ln_bwd, addresses, "yfs_layer_norm_bwd");
+    take(yfs.ln_ws, addresses, "yfs_layer_norm_bwd_workspace_bytes");
+    take(yfs.drop_fwd, addresses, "yfs_dropout_fwd");
+    take(yfs.drop_bwd, addresses, "yfs_dropout_bwd");
+    take(yfs.matmul, addresses, "yfs_fp8_matmul");
+    take(yfs.matmul_ws, addresses, "yfs_fp8_matmul_workspace_bytes");
+    g_error = error.inc_ref().ptr();   // for the life of the process
+}
+}  // namespace
+
+PYBIND11_MODULE(_binding, m) {
+    py::register_exception_translator([](std::exception_ptr p) {
+        try {
+            if (p) std::rethrow_exception(p);
+        } catch (const YfsException& e) {
+            PyErr_SetString(g_error ? g_error : PyExc_RuntimeError, e.what());
+        }
+    });
+    m.def("init", &init);
+    m.def("layer_norm", &layer_norm);
+    m.def("dropout", &dropout);
+    m.def("fp8_matmul", &fp8_matmul);
+}

@@ -112,14 +112,6 @@ def _bias(b, n, what):
     return b if b.is_contiguous() else b.contiguous()
 
 
-def _slope(slope, what):
-    slope = 1.0 if slope is None else float(slope)
-    if not 0.0 <= slope <= 1.0:
-        raise L.YfsError(f"{what}: slope must lie in [0, 1], got {slope}")
-    return slope
-
-
-@torch.no_grad()
 def fp8_matmul(x, w, bias=None, slope=None, out_dtype=None):
     """y [..., n] = leaky(Q(x) W^T + bias) for x [..., k] (fp32, bf16 or fp16; quantised by rows inside the call) and an
     ``Fp8Tensor`` w [n, k].  ``slope``: of a LeakyReLU behind the product (None: none).  ``out_dtype``: fp32, bf16 or fp16
@@ -127,25 +119,7 @@ def fp8_matmul(x, w, bias=None, slope=None, out_dtype=None):
     about 16 bits behind its largest product, 1 / 64 of the output's own rounding.  Not differentiable: see ``fp8_linear``."""
     if not isinstance(w, Fp8Tensor):
         raise L.YfsError(f"fp8_matmul: w must be an Fp8Tensor (quantize_fp8), got {type(w).__name__}")
-    if x.dim() == 0 or x.shape[-1] != w.k:
-        raise L.YfsError(f"fp8_matmul: x [..., {w.k}] expected, got {tuple(x.shape)}")
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in L.DTYPES:
-        raise L.YfsError(f"fp8_matmul: out_dtype must be fp32, bf16 or fp16, got {out_dtype}")
-    n, slope = w.data.shape[0], _slope(slope, "fp8_matmul")
-    x2, m, ld = _matrix(x.detach(), "fp8_matmul")
-    b = _bias(bias, n, "fp8_matmul")
-    L.require_cuda(x, w.data, w.scale, bias)
-    y = torch.empty(x.shape[:-1] + (n,), device=x.device, dtype=out_dtype)
-    if m == 0:
-        return y
-    lib = L.lib()
-    nbytes = lib.yfs_fp8_matmul_workspace_bytes(m, n, w.k)
-    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
-    with L.on_device("fp8_matmul", x2, w.data, w.scale, b) as stream:
-        L.check(lib.yfs_fp8_matmul(x2.data_ptr(), L.DTYPES[x2.dtype], ld, w.data.data_ptr(), w.scale.data_ptr(), _p(b), y.data_ptr(),
-                                   L.DTYPES[out_dtype], m, n, w.k, slope, ws.data_ptr(), nbytes, stream), "yfs_fp8_matmul")
-    return y
+    return (L._binding or L.binding()).fp8_matmul(x, w.data, w.scale, w.k, bias, slope, out_dtype)
 
 
 def _quantize_rows(x, rows, cols, colsum=False):
