@@ -374,6 +374,20 @@ size_t yfs_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int yfs_fp8_gemm(const void *aq, const void *a_scale, const void *bq, const void *b_scale, int b_row_scales, const float *bias,
                  void *out, int out_dtype, int64_t M, int64_t N, int64_t K, float slope, int accumulate, void *workspace,
                  size_t workspace_bytes, void *stream);
+/* A linear layer's training step, w [N, K] quantised in the call: y = Q(x) Q(w)^T + bias; dx = Q(dy) Q(w), dw (+)= Q(dy^T)
+ * Q(x^T)^T, db (+)= sum over rows of dy.  `needs`: which gradients the backward pass will be asked for (the same value in
+ * both calls; db alone needs no product: sum dy).  `saved` (256-byte aligned, like the workspaces) goes from the forward to
+ * the backward call: the transposed 8-bit operands, not x and w. */
+enum { YFS_NEED_DX = 1, YFS_NEED_DW = 2, YFS_NEED_DB = 4 };
+size_t yfs_fp8_linear_saved_bytes(int64_t M, int64_t N, int64_t K, int needs);
+size_t yfs_fp8_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K);
+size_t yfs_fp8_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int needs);
+int yfs_fp8_linear_fwd(const void *x, int x_dtype, int64_t ldx, const void *w, int w_dtype, int64_t ldw, const float *bias,
+                       void *y, int y_dtype, int64_t M, int64_t N, int64_t K, int needs, void *saved, size_t saved_bytes,
+                       void *workspace, size_t workspace_bytes, void *stream);
+int yfs_fp8_linear_bwd(const void *dy, int dy_dtype, int64_t lddy, void *dx, int dx_dtype, float *dw, int accumulate_w,
+                       float *db, int accumulate_b, int64_t M, int64_t N, int64_t K, int needs, const void *saved,
+                       size_t saved_bytes, void *workspace, size_t workspace_bytes, void *stream);
 /* The serving form: x [M, K] in `x_dtype` is quantised by rows in the workspace and multiplied by a stored weight. */
 size_t yfs_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int yfs_fp8_matmul(const void *x, int x_dtype, int64_t ld, const void *wq, const void *w_scale, const float *bias, void *y,

@@ -121,6 +121,31 @@ def test_refusals_of_the_library():
     assert lib.yfs_fp8_matmul(p, 1, 200, p, p, None, p, 1, 30, 40, 200, 1.0, p + 16, need, None) == -3
     assert lib.yfs_fp8_matmul_workspace_bytes(0, 1, 1) == 0 and lib.yfs_fp8_gemm_workspace_bytes(1, big, 1) == 0
     assert lib.yfs_fp8_colsum(p, 0, 8, p, 0, None) == -1
+    fwd, saved = lib.yfs_fp8_linear_fwd_workspace_bytes(5, 6, 7), lib.yfs_fp8_linear_saved_bytes(5, 6, 7, 3)
+    bwd = lib.yfs_fp8_linear_bwd_workspace_bytes(5, 6, 7, 7)
+    assert fwd and saved and bwd and lib.yfs_fp8_linear_saved_bytes(5, 6, 7, 0) == 0 and lib.yfs_fp8_linear_saved_bytes(0, 6, 7, 3) == 0
+    call = lambda y, needs, sb, wb: lib.yfs_fp8_linear_fwd(p, 1, 7, p, 0, 7, None, y, 1, 5, 6, 7, needs, p, sb, p, wb, None)   # noqa: E731
+    assert call(None, 3, saved, fwd) == -1 and call(p, 3, saved - 1, fwd) == -3 and call(p, 3, saved, fwd - 1) == -3
+    back = lambda dx, dw, db, needs, wb: lib.yfs_fp8_linear_bwd(p, 1, 6, dx, 1, dw, 0, db, 0, 5, 6, 7, needs, p, 1 << 20, p, wb, None)   # noqa: E731
+    assert back(p, p, None, 7, bwd) == -1 and back(None, p, p, 7, bwd) == -1 and back(None, None, p, 4, bwd) == -1
+    assert back(p, p, p, 7, bwd - 1) == -3
+
+
+def _quantize_rows(x, rows, cols, colsum=False):
+    """yfs_fp8_quantize_rows: x by rows and / or its transpose by rows, with packed scales, and the tile column sums."""
+    from yolo_from_scratch_amd import _lib as L
+    (m, k), dev, lib = x.shape, x.device, L.lib()
+    pad = lambda n: (n + 127) // 128 * 128   # noqa: E731
+    e4, u8 = torch.float8_e4m3fn, torch.uint8
+    q = torch.empty(m, pad(k), device=dev, dtype=e4) if rows else None
+    s = torch.empty(lib.yfs_fp8_packed_scale_bytes(m, k), device=dev, dtype=u8) if rows else None
+    qt = torch.empty(k, pad(m), device=dev, dtype=e4) if cols else None
+    st = torch.empty(lib.yfs_fp8_packed_scale_bytes(k, m), device=dev, dtype=u8) if cols else None
+    cs = torch.empty(pad(m) // 128, k, device=dev, dtype=torch.float32) if colsum else None
+    p = lambda t: t.data_ptr() if t is not None else None   # noqa: E731
+    L.check(lib.yfs_fp8_quantize_rows(x.data_ptr(), L.DTYPES[x.dtype], x.stride(0), m, k, p(q), p(s), p(qt), p(st), p(cs),
+                                      torch.cuda.current_stream().cuda_stream), "yfs_fp8_quantize_rows")
+    return q, s, qt, st, cs
 
 
 # ---- GPU: quantisers -------------------------------------------------------------------------------------------------
@@ -158,14 +183,14 @@ def test_quantisers(rows, cols, dtype):
     wide = torch.zeros(rows, cols + 9, dtype=x.dtype, device=DEV)
     wide[:, 5:5 + cols] = xd
     for src in (xd, wide[:, 5:5 + cols]):                    # dense, and rows at odd offsets with a stride of their own
-        q, s, qt, st, cs = f8._quantize_rows(src, True, True, True)
+        q, s, qt, st, cs = _quantize_rows(src, True, True, True)
         kb, mb = (cols + 127) // 128, (rows + 127) // 128
         for got, packed, arr, n, blocks in ((q, s, xn, rows, kb), (qt, st, xn.T, cols, mb)):
             ref, e = hr.quantize(arr, 1, 128)
             assert np.array_equal(_unpack_scales(packed, n, blocks), e)
             vals = _np(got.float())
             assert np.array_equal(vals[:, : arr.shape[1]], ref, equal_nan=True) and (vals[:, arr.shape[1]:] == 0).all()
-        alone = f8._quantize_rows(src, True, False)[0], f8._quantize_rows(src, False, True)[2]
+        alone = _quantize_rows(src, True, False)[0], _quantize_rows(src, False, True)[2]
         assert torch.equal(alone[0].view(torch.uint8), q.view(torch.uint8)) and torch.equal(alone[1].view(torch.uint8), qt.view(torch.uint8))
         finite = np.isfinite(xn).all(0)
         _close(_np(cs.double().sum(0))[finite], xn.sum(0)[finite], (128 * 2.0 ** -24 * np.abs(xn).sum(0) + 1e-40)[finite], "column sums")

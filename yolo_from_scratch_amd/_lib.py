@@ -28,7 +28,8 @@ def lib():
                      "yfs_conv2d_fwd_workspace_bytes", "yfs_conv2d_dgrad_workspace_bytes",
                      "yfs_conv2d_stem_wgrad_workspace_bytes", "yfs_single_box_loss_workspace_bytes",
                      "yfs_mask_to_boxes_workspace_bytes", "yfs_layer_norm_bwd_workspace_bytes",
-                     "yfs_fp8_packed_scale_bytes", "yfs_fp8_gemm_workspace_bytes", "yfs_fp8_matmul_workspace_bytes"):
+                     "yfs_fp8_packed_scale_bytes", "yfs_fp8_gemm_workspace_bytes", "yfs_fp8_matmul_workspace_bytes",
+                     "yfs_fp8_linear_saved_bytes", "yfs_fp8_linear_fwd_workspace_bytes", "yfs_fp8_linear_bwd_workspace_bytes"):
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = ctypes.c_size_t
         _declare(_lib)
@@ -49,6 +50,11 @@ _SIGNATURES = {
     "yfs_fp8_gemm": "pppp" "i" "p" "pi" "lll" "fi" "pz" "p",
     "yfs_fp8_matmul_workspace_bytes": "lll",
     "yfs_fp8_matmul": "pil" "pp" "p" "pi" "lll" "f" "pz" "p",
+    "yfs_fp8_linear_saved_bytes": "llli",
+    "yfs_fp8_linear_fwd_workspace_bytes": "lll",
+    "yfs_fp8_linear_bwd_workspace_bytes": "llli",
+    "yfs_fp8_linear_fwd": "pil" "pil" "p" "pi" "lll" "i" "pz" "pz" "p",
+    "yfs_fp8_linear_bwd": "pil" "pi" "pi" "pi" "lll" "i" "pz" "pz" "p",
     "yfs_fp8_colsum": "pllp" "i" "p",
     "yfs_dropout_fwd": "ppl" "ff" "u" "p" "i" "p",
     "yfs_dropout_bwd": "pppl" "ff" "u" "p" "i" "p",

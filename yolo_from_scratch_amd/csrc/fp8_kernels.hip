@@ -936,3 +936,122 @@ YFS_API int yfs_fp8_colsum(const float* part, int64_t tiles, int64_t K, float* o
     YFS_CHECK_LAUNCH("colsum_kernel");
     return YFS_OK;
 }
+
+// ---- a linear layer's training step ----------------------------------------------------------------------------------
+namespace {
+// consecutive pieces of one buffer, each 256-byte aligned
+struct Pieces {
+    unsigned char* base;
+    size_t used = 0;
+    unsigned char* take(size_t bytes) {
+        unsigned char* p = base + used;
+        used += align256(bytes);
+        return p;
+    }
+};
+// What the backward pass multiplies: the weight's blocks transposed (for dx), x's columns in blocks of 128 rows (for dw).
+struct Saved {
+    unsigned char *wqt = nullptr, *wst = nullptr, *xqt = nullptr, *xst = nullptr;
+    size_t bytes;
+    Saved(void* buf, long long M, long long N, long long K, int needs) {
+        Pieces p{(unsigned char*)buf};
+        if (needs & YFS_NEED_DX) {
+            wqt = p.take((size_t)(K * pad128(N)));
+            wst = p.take((size_t)(yfs_cdiv(K, 128) * yfs_cdiv(N, 128)));
+        }
+        if (needs & YFS_NEED_DW) {
+            xqt = p.take((size_t)(K * pad128(M)));
+            xst = p.take((size_t)packed_bytes(K, yfs_cdiv(M, 128)));
+        }
+        bytes = p.used;
+    }
+};
+struct ForwardSpace {
+    unsigned char *wq, *ws, *xq, *xs, *part;
+    size_t part_bytes, bytes;
+    ForwardSpace(void* buf, long long M, long long N, long long K) {
+        Pieces p{(unsigned char*)buf};
+        wq = p.take((size_t)(N * pad128(K)));
+        ws = p.take((size_t)(yfs_cdiv(N, 128) * yfs_cdiv(K, 128)));
+        xq = p.take((size_t)(M * pad128(K)));
+        xs = p.take((size_t)packed_bytes(M, yfs_cdiv(K, 128)));
+        part_bytes = yfs_fp8_gemm_workspace_bytes(M, N, K);
+        part = p.take(part_bytes);
+        bytes = p.used;
+    }
+};
+struct BackwardSpace {
+    unsigned char *dq = nullptr, *ds = nullptr, *dqt = nullptr, *dst = nullptr, *part;
+    float* colsum = nullptr;
+    size_t part_bytes = 0, bytes;
+    BackwardSpace(void* buf, long long M, long long N, long long K, int needs) {
+        Pieces p{(unsigned char*)buf};
+        if (needs & YFS_NEED_DX) {
+            dq = p.take((size_t)(M * pad128(N)));
+            ds = p.take((size_t)packed_bytes(M, yfs_cdiv(N, 128)));
+            part_bytes = yfs_fp8_gemm_workspace_bytes(M, K, N);
+        }
+        if (needs & YFS_NEED_DW) {
+            dqt = p.take((size_t)(N * pad128(M)));
+            dst = p.take((size_t)packed_bytes(N, yfs_cdiv(M, 128)));
+            const size_t b = yfs_fp8_gemm_workspace_bytes(N, K, M);
+            part_bytes = b > part_bytes ? b : part_bytes;
+        }
+        if (needs & YFS_NEED_DB) colsum = (float*)p.take((size_t)(yfs_cdiv(M, 128) * N * sizeof(float)));
+        part = p.take(part_bytes);   // the two products use it one after the other
+        bytes = p.used;
+    }
+};
+bool sizes_ok(long long M, long long N, long long K) { return M > 0 && N > 0 && K > 0 && M <= kMost && N <= kMost && K <= kMost; }
+bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255) == 0; }
+}  // namespace
+
+YFS_API size_t yfs_fp8_linear_saved_bytes(int64_t M, int64_t N, int64_t K, int needs) {
+    return sizes_ok(M, N, K) ? Saved(nullptr, M, N, K, needs).bytes : 0;
+}
+YFS_API size_t yfs_fp8_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    return sizes_ok(M, N, K) ? ForwardSpace(nullptr, M, N, K).bytes : 0;
+}
+YFS_API size_t yfs_fp8_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int needs) {
+    return sizes_ok(M, N, K) ? BackwardSpace(nullptr, M, N, K, needs).bytes : 0;
+}
+
+YFS_API int yfs_fp8_linear_fwd(const void* x, int x_dtype, int64_t ldx, const void* w, int w_dtype, int64_t ldw, const float* bias, void* y,
+                               int y_dtype, int64_t M, int64_t N, int64_t K, int needs, void* saved, size_t saved_bytes, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+    YFS_REQUIRE(x && w && y, YFS_ERR_INVALID_ARG, "yfs_fp8_linear_fwd: null pointer");
+    REQUIRE_SIZES("yfs_fp8_linear_fwd", M, N, K);
+    const Saved k(saved, M, N, K, needs);
+    const ForwardSpace f(workspace, M, N, K);
+    YFS_REQUIRE(workspace && workspace_bytes >= f.bytes && aligned256(workspace), YFS_ERR_WORKSPACE,
+                "yfs_fp8_linear_fwd: workspace needs %zu bytes, 256-byte aligned", f.bytes);
+    YFS_REQUIRE(k.bytes == 0 || (saved && saved_bytes >= k.bytes && aligned256(saved)), YFS_ERR_WORKSPACE,
+                "yfs_fp8_linear_fwd: saved needs %zu bytes, 256-byte aligned", k.bytes);
+    int rc = yfs_fp8_quantize_weight(w, w_dtype, ldw, N, K, f.wq, f.ws, k.wqt, k.wst, stream);
+    if (rc == YFS_OK) rc = yfs_fp8_quantize_rows(x, x_dtype, ldx, M, K, f.xq, f.xs, k.xqt, k.xst, nullptr, stream);
+    if (rc == YFS_OK)
+        rc = yfs_fp8_gemm(f.xq, f.xs, f.wq, f.ws, 0, bias, y, y_dtype, M, N, K, 1.0f, 0, f.part, f.part_bytes, stream);
+    return rc;
+}
+
+YFS_API int yfs_fp8_linear_bwd(const void* dy, int dy_dtype, int64_t lddy, void* dx, int dx_dtype, float* dw, int accumulate_w, float* db,
+                               int accumulate_b, int64_t M, int64_t N, int64_t K, int needs, const void* saved, size_t saved_bytes,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+    YFS_REQUIRE(dy && !dx == !(needs & YFS_NEED_DX) && !dw == !(needs & YFS_NEED_DW) && !db == !(needs & YFS_NEED_DB), YFS_ERR_INVALID_ARG,
+                "yfs_fp8_linear_bwd: null pointer, or an output that `needs` does not ask for");
+    YFS_REQUIRE(needs & (YFS_NEED_DX | YFS_NEED_DW), YFS_ERR_INVALID_ARG, "yfs_fp8_linear_bwd: neither dx nor dw is asked for");
+    REQUIRE_SIZES("yfs_fp8_linear_bwd", M, N, K);
+    const Saved k(const_cast<void*>(saved), M, N, K, needs);
+    const BackwardSpace f(workspace, M, N, K, needs);
+    YFS_REQUIRE(workspace && workspace_bytes >= f.bytes && aligned256(workspace), YFS_ERR_WORKSPACE,
+                "yfs_fp8_linear_bwd: workspace needs %zu bytes, 256-byte aligned", f.bytes);
+    YFS_REQUIRE(saved && saved_bytes >= k.bytes && aligned256(saved), YFS_ERR_WORKSPACE,
+                "yfs_fp8_linear_bwd: saved needs %zu bytes, 256-byte aligned", k.bytes);
+    int rc = yfs_fp8_quantize_rows(dy, dy_dtype, lddy, M, N, f.dq, f.ds, f.dqt, f.dst, f.colsum, stream);
+    if (rc == YFS_OK && dx)
+        rc = yfs_fp8_gemm(f.dq, f.ds, k.wqt, k.wst, 0, nullptr, dx, dx_dtype, M, K, N, 1.0f, 0, f.part, f.part_bytes, stream);
+    if (rc == YFS_OK && dw)
+        rc = yfs_fp8_gemm(f.dqt, f.dst, k.xqt, k.xst, 1, nullptr, dw, YFS_F32, N, K, M, 1.0f, accumulate_w, f.part, f.part_bytes, stream);
+    if (rc == YFS_OK && db) rc = yfs_fp8_colsum(f.colsum, yfs_cdiv(M, 128), N, db, accumulate_b, stream);
+    return rc;
+}

@@ -122,99 +122,78 @@ def fp8_matmul(x, w, bias=None, slope=None, out_dtype=None):
     return (L._binding or L.binding()).fp8_matmul(x, w.data, w.scale, w.k, bias, slope, out_dtype)
 
 
-def _quantize_rows(x, rows, cols, colsum=False):
-    """x [m, k] -> (q, scales) by rows of 128 columns and (q, scales) of the transpose by 128 rows, either may be left out, and
-    the sums of x over tiles of 128 rows."""
-    x2, m, ld = _matrix(x.detach(), "fp8_linear")
-    k, dev, lib = x2.shape[1], x2.device, L.lib()
-    e4, u8 = torch.float8_e4m3fn, torch.uint8
-    q = torch.empty(m, _pad(k), device=dev, dtype=e4) if rows else None
-    s = torch.empty(lib.yfs_fp8_packed_scale_bytes(m, k), device=dev, dtype=u8) if rows else None
-    qt = torch.empty(k, _pad(m), device=dev, dtype=e4) if cols else None
-    st = torch.empty(lib.yfs_fp8_packed_scale_bytes(k, m), device=dev, dtype=u8) if cols else None
-    cs = torch.empty(_pad(m) // BLOCK, k, device=dev, dtype=torch.float32) if colsum else None
-    with L.on_device("fp8_linear", x2) as stream:
-        L.check(lib.yfs_fp8_quantize_rows(x2.data_ptr(), L.DTYPES[x2.dtype], ld, m, k, _p(q), _p(s), _p(qt), _p(st), _p(cs), stream),
-                "yfs_fp8_quantize_rows")
-    return q, s, qt, st, cs
-
-
-def _gemm(aq, a_s, bq, b_s, row_scales, bias, out, m, n, k, accumulate=False):
-    lib = L.lib()
-    nbytes = lib.yfs_fp8_gemm_workspace_bytes(m, n, k)
-    ws = torch.empty(nbytes, device=out.device, dtype=torch.uint8) if nbytes else None
-    with L.on_device("fp8_linear", aq, bq, bias, out) as stream:
-        L.check(lib.yfs_fp8_gemm(aq.data_ptr(), a_s.data_ptr(), bq.data_ptr(), b_s.data_ptr(), row_scales, _p(bias), out.data_ptr(),
-                                 L.DTYPES[out.dtype], m, n, k, 1.0, int(accumulate), _p(ws), nbytes, stream), "yfs_fp8_gemm")
-    return out
-
-
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         n, k = weight.shape
         need_x, need_w, need_b = ctx.needs_input_grad
-        m = x.numel() // k
-        ctx.meta = (x.shape, x.dtype, m, n, k, bias.dtype if bias is not None else None)
-        ctx.wb = (weight, bias)          # for their gradient sinks; their values are not read again
-        y = torch.empty(x.shape[:-1] + (n,), device=x.device, dtype=x.dtype)
+        x2, m, ldx = _matrix(x, "fp8_linear")
+        w2, _, ldw = _matrix(weight, "fp8_linear")
+        # db alone is a sum of dy: nothing is kept for it
+        needs = (1 if need_x else 0) + (2 if need_w else 0) + (4 if need_b and (need_x or need_w) else 0)
+        ctx.meta = (x.shape, x.dtype, m, n, k, needs)
+        ctx.wb = (weight, bias)          # for their gradient sinks and types; their values are not read again
+        y = x.new_empty(x.shape[:-1] + (n,))
         if m == 0:
-            ctx.save_for_backward(None, None, None, None)
             return y
-        wq, ws, wqt, wst = _quantize_weight(weight, need_x)
-        xq, xs, xqt, xst, _ = _quantize_rows(x, True, need_w)
-        _gemm(xq, xs, wq, ws, 0, _bias(bias, n, "fp8_linear"), y, m, n, k)
-        # what the backward pass multiplies: the weight's blocks transposed, x's columns in blocks of 128 rows (8 bits each)
-        ctx.save_for_backward(wqt, wst, xqt, xst)
+        lib = L.lib()
+        saved_bytes = lib.yfs_fp8_linear_saved_bytes(m, n, k, needs)
+        space_bytes = lib.yfs_fp8_linear_fwd_workspace_bytes(m, n, k)
+        saved = x.new_empty(saved_bytes, dtype=torch.uint8) if saved_bytes else None
+        space = x.new_empty(space_bytes, dtype=torch.uint8)
+        b = _bias(bias, n, "fp8_linear")
+        with L.on_device("fp8_linear", x2, w2, b) as stream:
+            L.check(lib.yfs_fp8_linear_fwd(x2.data_ptr(), L.DTYPES[x2.dtype], ldx, w2.data_ptr(), L.DTYPES[w2.dtype], ldw, _p(b),
+                                           y.data_ptr(), L.DTYPES[y.dtype], m, n, k, needs, _p(saved), saved_bytes,
+                                           space.data_ptr(), space_bytes, stream), "yfs_fp8_linear_fwd")
+        if saved is not None:
+            ctx.save_for_backward(saved)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         from .train import write_grad
-        wqt, wst, xqt, xst = ctx.saved_tensors
-        shape, dtype, m, n, k, bias_dtype = ctx.meta
+        shape, dtype, m, n, k, needs = ctx.meta
         weight, bias = ctx.wb
         need_x, need_w, need_b = ctx.needs_input_grad
-        dev = dy.device
         if m == 0:
-            return (torch.empty(shape, device=dev, dtype=dtype) if need_x else None,
-                    torch.zeros_like(weight) if need_w else None, torch.zeros_like(bias) if need_b else None)
-        dy2 = _matrix(dy if dy.dtype in L.DTYPES else dy.to(dtype), "fp8_linear")[0]
-        dq, ds, dqt, dst, colsum = _quantize_rows(dy2, need_x, need_w, need_b) if (need_x or need_w) else (None,) * 5
-        dx = dw = db = None
-        if need_x:
-            dx = _gemm(dq, ds, wqt, wst, 0, None, torch.empty(shape, device=dev, dtype=dtype), m, k, n)
-
-        def put_w(sink, acc):
+            return (dy.new_empty(shape) if need_x else None, torch.zeros_like(weight) if need_w else None,
+                    torch.zeros_like(bias) if need_b else None)
+        dy2, _, ldy = _matrix(dy, "fp8_linear")
+        if not needs:
+            def put_alone(sink, acc):
+                total = dy2.float().sum(0).to(bias.dtype)
+                if sink is None:
+                    return total
+                sink.add_(total) if acc else sink.copy_(total)
+            return None, None, write_grad(bias, put_alone) if need_b else None
+        (saved,) = ctx.saved_tensors
+        dx = dy.new_empty(shape) if need_x else None
+        # a gradient sink (train.FlatSGD) that the kernels can write is written by them; any other gets the result afterwards
+        outs, results = [], []
+        for param, shape_, need in ((weight, (n, k), need_w), (bias, (n,), need_b)):
+            sink = getattr(param, "_yfs_grad_sink", None) if need else None
             direct = sink is not None and sink.dtype == torch.float32 and sink.is_contiguous()
-            out = _gemm(dqt, dst, xqt, xst, 1, None, sink if direct else torch.empty(n, k, device=dev, dtype=torch.float32), n, k, m,
-                        acc and direct)
-            if sink is None:
-                return out if weight.dtype == torch.float32 else out.to(weight.dtype)
-            if not direct:
-                sink.add_(out) if acc else sink.copy_(out)
-
-        def put_b(sink, acc):
-            if colsum is None:
-                total = dy2.float().sum(0)
-            else:
-                direct = sink is not None and sink.dtype == torch.float32 and sink.is_contiguous()
-                total = sink if direct else torch.empty(n, device=dev, dtype=torch.float32)
-                with L.on_device("fp8_linear", colsum, total) as stream:
-                    L.check(L.lib().yfs_fp8_colsum(colsum.data_ptr(), colsum.shape[0], n, total.data_ptr(), int(acc and direct), stream),
-                            "yfs_fp8_colsum")
-                if direct:
-                    return None
-            if sink is None:
-                return total if bias_dtype == torch.float32 else total.to(bias_dtype)
-            sink.add_(total) if acc else sink.copy_(total)
-        if need_w:
-            dw = write_grad(weight, put_w)
-        if need_b:
-            db = write_grad(bias, put_b)
+            acc = direct and not param._yfs_grad_fresh
+            outs.append(((sink if direct else dy.new_empty(shape_, dtype=torch.float32)) if need else None, acc, direct))
+        (dw, acc_w, _), (db, acc_b, _) = outs
+        lib = L.lib()
+        nbytes = lib.yfs_fp8_linear_bwd_workspace_bytes(m, n, k, needs)
+        space = dy.new_empty(nbytes, dtype=torch.uint8)
+        with L.on_device("fp8_linear", dy2, saved, dw, db) as stream:
+            L.check(lib.yfs_fp8_linear_bwd(dy2.data_ptr(), L.DTYPES[dy2.dtype], ldy, _p(dx), L.DTYPES[dtype], _p(dw), int(acc_w), _p(db),
+                                           int(acc_b), m, n, k, needs, saved.data_ptr(), saved.numel(), space.data_ptr(), nbytes,
+                                           stream), "yfs_fp8_linear_bwd")
+        for param, (out, acc, direct) in zip((weight, bias), outs):
+            def put(sink, accumulate):
+                if sink is None:
+                    return out if out.dtype == param.dtype else out.to(param.dtype)
+                if not direct:
+                    sink.add_(out) if accumulate else sink.copy_(out)
+            results.append(write_grad(param, put) if out is not None else None)
         ctx.wb = None
-        return dx, dw, db
+        return dx, results[0], results[1]
 
 
 def fp8_linear(x, weight, bias=None):
