@@ -560,9 +560,15 @@ class YoloRegressorModel(nn.Module):
     ``head_out`` = 4 reproduces the reference ([xc,yc,w,h]); 7*7*30 = 1470 gives the YOLOv1 S=7,B=2,C=20
     head that BASELINE.json's train-step config uses (build-defined: the reference stops at 4 outputs).
     ``image_size`` sizes fc.1 the way the reference's 448 dummy forward does (:255-257).
+
+    Two forms of the head that the reference does not have, with the indices and keys of fc.1 and fc.4 unchanged:
+    ``head_norm`` puts a layer norm between fc.1 and its activation (fc.2: HipLayerNorm; README.md:30 names normalisation as
+    the next step), ``head_fp8`` multiplies fc.1 and fc.4 in 8 bits with block scales (Fp8Linear).  In both, activation and
+    dropout are one kernel without a stored mask (fc.3: HipDropout).  ``fp8_ops.freeze_fp8(model)`` turns the linear layers
+    of any form into 8-bit ones for serving.
     """
 
-    def __init__(self, head_out=4, image_size=448, p_drop=0.2):
+    def __init__(self, head_out=4, image_size=448, p_drop=0.2, head_norm=False, head_fp8=False):
         super().__init__()
         pool = HipMaxPool2d
         self.feat = Backbone(
@@ -581,6 +587,19 @@ class YoloRegressorModel(nn.Module):
         for m in self.feat:
             hw = hw // 2 if isinstance(m, HipMaxPool2d) else co.out_hw(hw, hw, m[0].kernel_size, m[0].stride)[0]
         flat = 1024 * hw * hw
+        if head_norm or head_fp8:
+            from .drop_ops import HipDropout
+            from .fp8_ops import Fp8Linear
+            from .norm_ops import HipLayerNorm
+            linear = Fp8Linear if head_fp8 else HipLinear
+            self.fc = nn.Sequential(
+                nn.Flatten(),
+                linear(flat, 4096),
+                HipLayerNorm(4096) if head_norm else FusedLeakyReLU(SLOPE),
+                HipDropout(p_drop, slope=SLOPE),
+                linear(4096, head_out),
+            )
+            return
         self.fc = nn.Sequential(
             nn.Flatten(),
             HipLinear(flat, 4096, fused_act=SLOPE if _FUSE_FC else None),
