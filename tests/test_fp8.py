@@ -104,6 +104,7 @@ def test_refusals_of_the_library():
     import yolo_from_scratch_amd as y
     lib, p = y.lib(), 4096
     big = 1 << 23
+    assert lib.yfs_fp8_gemm(p, p, p, p, 1, None, p, 1, 8, 8, 8, 1.0, 0, None, 0, None) == -2      # row scales on both sides: fp32 only
     assert lib.yfs_fp8_quantize_weight(None, 0, 8, 8, 8, p, p, None, None, None) == -1
     assert lib.yfs_fp8_quantize_weight(p, 0, 8, 8, 8, p, p, p, None, None) == -1
     assert lib.yfs_fp8_quantize_weight(p, 0, 8, big, 8, p, p, None, None, None) == -1
@@ -239,11 +240,15 @@ def test_matmul(m, n, k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k,kernel", [(1, 4096, 50176, "fp8_rows_kernel"), (3, 40, 50176, "fp8_rows_kernel"),
-                                          (16, 1470, 4096, "fp8_rows_kernel"), (16, 512, 50176, "fp8_gemm_kernel<64"),
-                                          (64, 512, 50176, "fp8_gemm_kernel<64"), (1500, 1300, 1111, "fp8_gemm_kernel<128"),
-                                          (700, 2048, 4096, "fp8_gemm_kernel<128"), (4099, 4101, 640, "fp8_gemm8_kernel"),
-                                          (4352, 4096, 768, "fp8_gemm8_kernel"), (2100, 8300, 515, "fp8_gemm8_kernel"),
-                                          (8192, 2304, 2048, "fp8_gemm8_kernel")])
+                                          (16, 1470, 4096, "fp8_rows_kernel"), (16, 512, 50176, "fp8_gemm_kernel<64,128,splits"),
+                                          (64, 512, 50176, "fp8_gemm_kernel<64,128,splits"), (3, 70000, 300, "fp8_rows_kernel"),
+                                          (20, 40000, 300, "fp8_gemm_kernel<64,128,splits1>"),
+                                          (300, 2600, 1111, "fp8_gemm_kernel<64,64,splits1>"),
+                                          (1500, 1300, 1111, "fp8_gemm_kernel<64,128,splits1>"),
+                                          (2600, 2900, 500, "fp8_gemm_kernel<128,128,splits1>"),
+                                          (3000, 4096, 515, "fp8_gemm8_kernel<rest0>"), (4099, 4101, 640, "fp8_gemm8_kernel<rest259>"),
+                                          (4352, 4096, 768, "fp8_gemm8_kernel<rest256>"), (2100, 8300, 515, "fp8_gemm8_kernel<rest308>"),
+                                          (16300, 1100, 257, "fp8_gemm8_kernel<rest"), (8192, 2304, 2048, "fp8_gemm8_kernel")])
 def test_matmul_large_against_fp64_on_the_gpu(m, n, k, kernel):
     """Every kernel the size rule chooses, at ragged sizes and odd counts of blocks."""
     import yolo_from_scratch_amd as yfs
@@ -294,7 +299,8 @@ def test_shapes_strides_and_special_values():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 40, 200), (5, 129, 64), (64, 100, 300), (128, 128, 128), (130, 257, 131), (300, 64, 513)])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 40, 200), (5, 129, 64), (64, 100, 300), (128, 128, 128), (130, 257, 131), (300, 64, 513),
+                                   (40, 1300, 1500), (600, 1500, 1400)])
 def test_linear_forward_and_gradients(m, n, k, dtype):
     import yolo_from_scratch_amd as yfs
     t = DTYPES[dtype]

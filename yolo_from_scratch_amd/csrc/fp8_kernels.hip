@@ -28,9 +28,6 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 __host__ __device__ inline long long pad128(long long n) { return (n + 127) & ~127LL; }
 __host__ __device__ inline int groups64(long long rows) { return (int)((rows + 255) / 256 * 4); }
 __host__ __device__ inline long long packed_bytes(long long rows, long long kblocks) { return kblocks * groups64(rows) * 64; }
-__device__ __forceinline__ long long packed_at(long long row, long long kb, int groups) {
-    return (kb * groups + (row >> 6)) * 64 + (row & 15) * 4 + ((row & 63) >> 4);
-}
 
 // e of the smallest power of two with amax <= 448 * 2^e = 0.875 * 2^(e + 9); amax finite and >= 0
 __device__ __forceinline__ int scale_exponent(float amax) {
@@ -54,101 +51,53 @@ struct QuantArgs {
     long long ld, M, K;        // x [M, K], ld elements from row to row
     unsigned char *q, *s;      // [M, pad128(K)] and its scales (packed row scales, or [ceil(M/128), ceil(K/128)])
     unsigned char *qt, *st;    // the transpose [K, pad128(M)] and its scales
-    float* colsum;             // [ceil(M/128), K] sums of x over the rows of a tile, or NULL
+    float* colsum;             // [ceil(M/128), K] sums of x over 128 rows each, or NULL
     int groups, groups_t;      // 64-row groups of the packed planes of q and qt
+    int row_blocks;            // workgroups that quantise by rows
 };
 
-// One workgroup per 128 x 128 tile, 8 x 8 elements per thread.  BLOCK: one scale for the tile.  Otherwise ROWQ: a scale per
-// row; COLQ: a scale per column, written transposed.
-template <typename T, bool BLOCK, bool ROWQ, bool COLQ>
-__global__ void __launch_bounds__(256) quant_tile_kernel(QuantArgs g) {
-    __shared__ float red[4][128];
+// Weights: one workgroup and one scale per 128 x 128 tile, 8 x 8 elements per thread; the transpose leaves through LDS.
+template <typename T, bool COLQ>
+__global__ void __launch_bounds__(256) quant_block_kernel(QuantArgs g) {
+    __shared__ float red[4];
     __shared__ __attribute__((aligned(16))) unsigned char tile[COLQ ? 128 * 144 : 16];
     const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4, wave = threadIdx.x >> 6;
-    const long long kb = blockIdx.x, mb = blockIdx.y;
+    // Neighbouring workgroups take a patch of up to 32 tiles down by the rest across: rows of a power of two times an odd number
+    // of bytes meet few channels along one axis, whichever it is
+    const int across = (int)((g.K + 127) >> 7), down = (int)((g.M + 127) >> 7), grp = (int)blockIdx.x / (32 * across);
+    const int in = (int)blockIdx.x - grp * 32 * across, high = down - grp * 32 < 32 ? down - grp * 32 : 32;
+    const long long kb = in / high, mb = grp * 32 + in - (int)kb * high;
     const long long k0 = kb * 128 + cg * 8, m0 = mb * 128 + rg * 8;
-    float v[8][8];
+    const long long ldq = pad128(g.K), ldt = pad128(g.M);
+    float v[8][8], a = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) load_vec8((const T*)g.x + (m0 + i) * g.ld + k0, m0 + i < g.M ? g.K - k0 : 0, v[i]);
-    if (g.colsum) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float s = 0.0f;
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[i][j];
-            s += __shfl_xor(s, 16, 64);
-            s += __shfl_xor(s, 32, 64);
-            if ((threadIdx.x & 48) == 0) red[wave][cg * 8 + j] = s;
-        }
-        __syncthreads();
-        if (threadIdx.x < 128 && kb * 128 + threadIdx.x < g.K)
-            g.colsum[mb * g.K + kb * 128 + threadIdx.x] =
-                (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
-        __syncthreads();
+        for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(v[i][j]));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+    if ((threadIdx.x & 63) == 0) red[wave] = a;
+    __syncthreads();
+    const int e = scale_exponent(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    const float f = pow2(-e);
+    if (threadIdx.x == 0) {
+        g.s[mb * (ldq >> 7) + kb] = (unsigned char)(e + 127);
+        if (COLQ) g.st[kb * (ldt >> 7) + mb] = (unsigned char)(e + 127);
     }
-    const long long ldq = pad128(g.K), ldt = pad128(g.M);
-    int eb = 0;
-    if (BLOCK) {
-        float a = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(v[i][j]));
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
-        if ((threadIdx.x & 63) == 0) red[0][wave] = a;
-        __syncthreads();
-        eb = scale_exponent(fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])));
-        if (threadIdx.x == 0) {
-            if (ROWQ) g.s[mb * (ldq >> 7) + kb] = (unsigned char)(eb + 127);
-            if (COLQ) g.st[kb * (ldt >> 7) + mb] = (unsigned char)(eb + 127);
-        }
-    }
-    if (ROWQ) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            int e = eb;
-            if (!BLOCK) {
-                float a = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(v[i][j]));
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
-                e = scale_exponent(a);
-                if (cg == 0 && m0 + i < g.M) g.s[packed_at(m0 + i, kb, g.groups)] = (unsigned char)(e + 127);
-            }
-            const float f = pow2(-e);
-            const uint2 p = make_uint2(pack4(v[i][0] * f, v[i][1] * f, v[i][2] * f, v[i][3] * f),
-                                       pack4(v[i][4] * f, v[i][5] * f, v[i][6] * f, v[i][7] * f));
-            if (m0 + i < g.M) *reinterpret_cast<uint2*>(g.q + (m0 + i) * ldq + k0) = p;
-        }
+    for (int i = 0; i < 8; ++i) {
+        const uint2 p = make_uint2(pack4(v[i][0] * f, v[i][1] * f, v[i][2] * f, v[i][3] * f),
+                                   pack4(v[i][4] * f, v[i][5] * f, v[i][6] * f, v[i][7] * f));
+        if (m0 + i < g.M) *reinterpret_cast<uint2*>(g.q + (m0 + i) * ldq + k0) = p;
     }
     if (COLQ) {
-        if (!BLOCK) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float a = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) a = fmaxf(a, finite_abs(v[i][j]));
-                a = fmaxf(a, __shfl_xor(a, 16, 64));
-                a = fmaxf(a, __shfl_xor(a, 32, 64));
-                if ((threadIdx.x & 48) == 0) red[wave][cg * 8 + j] = a;
-            }
-            __syncthreads();
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            int e = eb;
-            if (!BLOCK) {
-                const int c = cg * 8 + j;
-                e = scale_exponent(fmaxf(fmaxf(red[0][c], red[1][c]), fmaxf(red[2][c], red[3][c])));
-                if (rg == 0 && k0 + j < g.K) g.st[packed_at(k0 + j, mb, g.groups_t)] = (unsigned char)(e + 127);
-            }
-            const float f = pow2(-e);
+        for (int j = 0; j < 8; ++j)
             *reinterpret_cast<uint2*>(tile + (cg * 8 + j) * 144 + rg * 8) =
                 make_uint2(pack4(v[0][j] * f, v[1][j] * f, v[2][j] * f, v[3][j] * f),
                            pack4(v[4][j] * f, v[5][j] * f, v[6][j] * f, v[7][j] * f));
-        }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -160,28 +109,86 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(QuantArgs g) {
     }
 }
 
-// By rows alone: 16 lanes x 8 elements per block, blocks of a row next to each other.
+// Activations and gradients.  The first row_blocks workgroups quantise by rows, 16 lanes x 8 elements per block, blocks of a row
+// next to each other (four rows per thread, whose scales fill a dword of the packed plane, were slower: 12544 x 4096 bf16 35 us
+// against 29, 5.3 TB/s).  The others take 128 rows x 64 columns: column sums, and the transpose by rows, through LDS.  The second
+// read of x comes from the caches; one 128 x 128 tile for both took 14 us where this takes 10 (64 x 50176 bf16): too few
+// workgroups with too long a chain of reductions each.
 template <typename T>
 __global__ void __launch_bounds__(256) quant_rows_kernel(QuantArgs g) {
-    const long long kblocks = (g.K + 127) >> 7, total = g.M * kblocks;
-    const int l = threadIdx.x & 15;
-    for (long long id = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); id < total; id += (long long)gridDim.x * 16) {
-        const long long m = id / kblocks, kb = id - m * kblocks, k = kb * 128 + l * 8;
-        float v[8], a = 0.0f;
-        load_vec8((const T*)g.x + m * g.ld + k, g.K - k, v);
+    __shared__ float top[4][64], sum[4][64];
+    __shared__ unsigned tile[64 * 33];   // [column][128 rows + 4 bytes]
+    if ((int)blockIdx.x < g.row_blocks) {
+        const long long kblocks = (g.K + 127) >> 7, total = g.M * kblocks;
+        const int l = threadIdx.x & 15;
+        for (long long id = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); id < total; id += (long long)g.row_blocks * 16) {
+            const long long m = id / kblocks, kb = id - m * kblocks, k = kb * 128 + l * 8;
+            float v[8], a = 0.0f;
+            load_vec8((const T*)g.x + m * g.ld + k, g.K - k, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(v[j]));
+            for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(v[j]));
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
-        const int e = scale_exponent(a);
-        if (l == 0) g.s[packed_at(m, kb, g.groups)] = (unsigned char)(e + 127);
-        const float f = pow2(-e);
-        *reinterpret_cast<uint2*>(g.q + m * kblocks * 128 + k) =
-            make_uint2(pack4(v[0] * f, v[1] * f, v[2] * f, v[3] * f), pack4(v[4] * f, v[5] * f, v[6] * f, v[7] * f));
+            for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+            const int e = scale_exponent(a);
+            if (l == 0) g.s[(kb * g.groups + (m >> 6)) * 64 + (m & 15) * 4 + ((m & 63) >> 4)] = (unsigned char)(e + 127);
+            const float f = pow2(-e);
+            *reinterpret_cast<uint2*>(g.q + m * kblocks * 128 + k) =
+                make_uint2(pack4(v[0] * f, v[1] * f, v[2] * f, v[3] * f), pack4(v[4] * f, v[5] * f, v[6] * f, v[7] * f));
+        }
+        return;
+    }
+    const long long strips = (g.K + 63) >> 6, id = (long long)blockIdx.x - g.row_blocks, mb = id / strips, strip = id - mb * strips, k0 = strip * 64;
+    const int cg = threadIdx.x & 7, rg = threadIdx.x >> 3, wave = threadIdx.x >> 6;
+    const long long m0 = mb * 128 + rg * 4, kc = k0 + cg * 8, ldt = pad128(g.M);
+    float v[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_vec8((const T*)g.x + (m0 + i) * g.ld + kc, m0 + i < g.M ? g.K - kc : 0, v[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float a = 0.0f, s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a = fmaxf(a, finite_abs(v[i][j]));
+            s += v[i][j];
+        }
+#pragma unroll
+        for (int o = 8; o < 64; o <<= 1) {
+            a = fmaxf(a, __shfl_xor(a, o, 64));
+            if (g.colsum) s += __shfl_xor(s, o, 64);
+        }
+        if ((threadIdx.x & 56) == 0) {
+            top[wave][cg * 8 + j] = a;
+            sum[wave][cg * 8 + j] = s;
+        }
+    }
+    __syncthreads();
+    if (g.colsum && threadIdx.x < 64 && k0 + threadIdx.x < g.K)
+        g.colsum[mb * g.K + k0 + threadIdx.x] = (sum[0][threadIdx.x] + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x]);
+    if (!g.qt) return;
+    auto exponent = [&](int c) { return scale_exponent(fmaxf(fmaxf(top[0][c], top[1][c]), fmaxf(top[2][c], top[3][c]))); };
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float f = pow2(-exponent(cg * 8 + j));
+        tile[(cg * 8 + j) * 33 + rg] = pack4(v[0][j] * f, v[1][j] * f, v[2][j] * f, v[3][j] * f);
+    }
+    if (threadIdx.x < 16) {   // the 64 columns are one line of the packed scales
+        unsigned bytes = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bytes |= (unsigned)(exponent(i * 16 + (int)threadIdx.x) + 127) << (8 * i);
+        *reinterpret_cast<unsigned*>(g.st + (mb * g.groups_t + strip) * 64 + threadIdx.x * 4) = bytes;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = i * 32 + (threadIdx.x >> 3), ch = threadIdx.x & 7;
+        if (k0 + c < g.K) {
+            const unsigned* t = tile + c * 33 + ch * 4;
+            *reinterpret_cast<uint4*>(g.qt + (k0 + c) * ldt + mb * 128 + ch * 16) = make_uint4(t[0], t[1], t[2], t[3]);
+        }
     }
 }
 
-// sums over the tiles of quant_tile_kernel's colsum, in tile order
+// sums over quant_rows_kernel's colsum, in the order of the rows
 __global__ void __launch_bounds__(256) colsum_kernel(const float* __restrict__ part, long long tiles, long long K,
                                                      float* __restrict__ out, int accumulate) {
     const long long k = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -191,23 +198,27 @@ __global__ void __launch_bounds__(256) colsum_kernel(const float* __restrict__ p
     out[k] = accumulate ? out[k] + s : s;
 }
 
-int quantize_rows_only(const QuantArgs& g, int dtype, hipStream_t s) {
-    const long long nb = yfs_cdiv(g.M * yfs_cdiv(g.K, 128), 16);
-    const dim3 grid((unsigned)(nb < 16384 ? nb : 16384));
+template <bool COLQ>
+int quantize_blocks(const QuantArgs& g, int dtype, hipStream_t s) {
+    YFS_REQUIRE(yfs_cdiv(g.K, 128) * yfs_cdiv(g.M, 128) < (1LL << 31) - 64, YFS_ERR_UNSUPPORTED, "yfs_fp8_quantize_weight: %lld x %lld is too large",
+                g.M, g.K);
+    const dim3 grid((unsigned)(yfs_cdiv(g.K, 128) * yfs_cdiv(g.M, 128)));
+    if (dtype == YFS_F32) quant_block_kernel<float, COLQ><<<grid, 256, 0, s>>>(g);
+    else if (dtype == YFS_BF16) quant_block_kernel<bf16_t, COLQ><<<grid, 256, 0, s>>>(g);
+    else quant_block_kernel<_Float16, COLQ><<<grid, 256, 0, s>>>(g);
+    YFS_CHECK_LAUNCH("quant_block_kernel");
+    return YFS_OK;
+}
+int quantize_rows(QuantArgs g, int dtype, hipStream_t s) {
+    const long long all = g.q ? yfs_cdiv(g.M * yfs_cdiv(g.K, 128), 16) : 0, rows = all < 16384 ? all : 16384;
+    const long long cols = g.qt || g.colsum ? yfs_cdiv(g.K, 64) * yfs_cdiv(g.M, 128) : 0;
+    g.row_blocks = (int)rows;
+    YFS_REQUIRE(rows + cols < (1LL << 31), YFS_ERR_UNSUPPORTED, "yfs_fp8_quantize_rows: %lld x %lld is too large", g.M, g.K);
+    const dim3 grid((unsigned)(g.row_blocks + cols));
     if (dtype == YFS_F32) quant_rows_kernel<float><<<grid, 256, 0, s>>>(g);
     else if (dtype == YFS_BF16) quant_rows_kernel<bf16_t><<<grid, 256, 0, s>>>(g);
     else quant_rows_kernel<_Float16><<<grid, 256, 0, s>>>(g);
     YFS_CHECK_LAUNCH("quant_rows_kernel");
-    return YFS_OK;
-}
-
-template <bool BLOCK, bool ROWQ, bool COLQ>
-int quantize(const QuantArgs& g, int dtype, hipStream_t s) {
-    const dim3 grid((unsigned)yfs_cdiv(g.K, 128), (unsigned)yfs_cdiv(g.M, 128));
-    if (dtype == YFS_F32) quant_tile_kernel<float, BLOCK, ROWQ, COLQ><<<grid, 256, 0, s>>>(g);
-    else if (dtype == YFS_BF16) quant_tile_kernel<bf16_t, BLOCK, ROWQ, COLQ><<<grid, 256, 0, s>>>(g);
-    else quant_tile_kernel<_Float16, BLOCK, ROWQ, COLQ><<<grid, 256, 0, s>>>(g);
-    YFS_CHECK_LAUNCH("quant_tile_kernel");
     return YFS_OK;
 }
 
@@ -221,6 +232,7 @@ struct GemmArgs {
     long long M, N;
     int kblocks, splits, per_split;
     int groups_a, groups_b;
+    long long row0;                // row of the scales' planes that a[0] is (a call for the last rows of a larger product)
     float slope;                   // 1: no activation
     int accumulate;                // fp32 output only: add to what is there
 };
@@ -251,26 +263,59 @@ __device__ __forceinline__ f32x4 mfma_fp8(const i32x8& a, const i32x8& b, f32x4 
 
 __device__ __forceinline__ float leaky(float v, float slope) { return v > 0.0f ? v : v * slope; }
 
+__device__ __forceinline__ f32x4 load4(const float* p, long long n, long long N) {   // p[n .. n + 3], zeros from N on
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (n + 4 <= N) __builtin_memcpy(&v, p + n, 16);
+    else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (n + r < N) v[r] = p[n + r];
+    }
+    return v;
+}
+__device__ __forceinline__ f32x4 act4(f32x4 v, f32x4 bias, float slope) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = leaky(v[r] + bias[r], slope);
+    return v;
+}
+
 // Four neighbouring outputs of row m: columns n .. n + 3, of which those below N exist
 template <typename TO>
 __device__ __forceinline__ void store4(const GemmArgs& g, long long m, long long n, f32x4 v) {
-    if (g.bias) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] += n + r < g.N ? g.bias[n + r] : 0.0f;
-    }
-    TO t[4];
+    const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+    v = act4(v, g.bias ? load4(g.bias, n, g.N) : none, g.slope);
     TO* o = (TO*)g.out + m * g.N + n;
-    if (sizeof(TO) == 4 && g.accumulate) {
+    TO t[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] += n + r < g.N ? (float)o[r] : 0.0f;
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) t[r] = (TO)leaky(v[r], g.slope);
+    for (int r = 0; r < 4; ++r) t[r] = (TO)(sizeof(TO) == 4 && g.accumulate && n + r < g.N ? v[r] + (float)o[r] : v[r]);
     if (n + 4 <= g.N) __builtin_memcpy(o, t, sizeof(t));
     else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (n + r < g.N) o[r] = t[r];
+    }
+}
+
+// A finished tile of BM x BN fp32 outputs leaves through LDS ([row][BN * 4 + 16 bytes]), whole rows at a time.  Straight from the
+// accumulators a wave would write 16 rows x 64 bytes at once, and rows of a power of two times an odd number of bytes all fall
+// on one channel of the L2 (50176 columns: 330 us for 822 MB, 157 through LDS).  16-bit outputs gain nothing by it.
+template <int BM, int BN, int NT>
+__device__ __forceinline__ void store_tile(const GemmArgs& g, const unsigned char* smem, long long m0, long long n0) {
+    constexpr int PER = BN / 4, PITCH = BN * 4 + 16;
+#pragma unroll 4
+    for (int id = threadIdx.x; id < BM * PER; id += NT) {
+        const int r = id / PER, ch = id % PER;
+        const long long m = m0 + r, n = n0 + ch * 4;
+        if (m >= g.M || n >= g.N) continue;
+        f32x4 t = *reinterpret_cast<const f32x4*>(smem + r * PITCH + ch * 16);
+        float* o = (float*)g.out + m * g.N + n;
+        if (g.accumulate) t += load4((const float*)g.out + m * g.N, n, g.N);
+        if (n + 4 <= g.N) __builtin_memcpy(o, &t, 16);
+        else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + j < g.N) o[j] = t[j];
+        }
     }
 }
 
@@ -341,7 +386,7 @@ __global__ void __launch_bounds__(64 * WM * WN) fp8_gemm_kernel(GemmArgs g) {
                                                      (unsigned)((r * 8 + srow) * ld) + chunk, so, 0, 0);
         }
         // each wave its own copy of the scales: 4 groups of 64 rows; groups behind the plane's end are not used
-        const long long ga = (long long)kb * g.groups_a + (m0 >> 6);
+        const long long ga = (long long)kb * g.groups_a + ((g.row0 + m0) >> 6);
         const __amdgpu_buffer_rsrc_t rs = rsrc(g.as + ga * 64, ((long long)g.kblocks * g.groups_a - ga) * 64);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(base + TILE + wave * 256), 4, (unsigned)lane * 4u, 0, 0, 0);
         if (ROWB) {
@@ -420,6 +465,22 @@ __global__ void __launch_bounds__(64 * WM * WN) fp8_gemm_kernel(GemmArgs g) {
             row(std::integral_constant<int, 3>());
         }
     }
+    if (sizeof(TO) == 4 && g.splits == 1) {
+        barrier();   // every wave has read its last fragments: the ring becomes the tile
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+            const int col = wn * FN * 16 + i * 16 + fk * 4;
+            const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+            const f32x4 bias = g.bias ? load4(g.bias, n0 + col, g.N) : none;
+#pragma unroll
+            for (int j = 0; j < FM; ++j)
+                *reinterpret_cast<f32x4*>(smem + (wm * FM * 16 + j * 16 + frow) * (BN * 4 + 16) + col * 4) = act4(acc[i][j], bias, g.slope);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        barrier();
+        store_tile<BM, BN, 64 * NW>(g, smem, m0, n0);
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
         const long long m = m0 + wm * FM * 16 + j * 16 + frow;
@@ -429,7 +490,7 @@ __global__ void __launch_bounds__(64 * WM * WN) fp8_gemm_kernel(GemmArgs g) {
             const long long n = n0 + wn * FN * 16 + i * 16 + fk * 4;
             if (n >= g.N) continue;
             if (g.splits > 1) store_part(g, blockIdx.z, m, n, acc[i][j]);
-            else store4<TO>(g, m, n, acc[i][j]);
+            else if constexpr (sizeof(TO) < 4) store4<TO>(g, m, n, acc[i][j]);
         }
     }
 }
@@ -563,7 +624,9 @@ __global__ void __launch_bounds__(512, 2) fp8_gemm8_kernel(GemmArgs g) {
         block(t + 1, std::integral_constant<int, 1>());
     }
     if (wm == 0) barrier();
-    wait_vm<0>();
+    wait_vm<0>();   // (the loads of no bytes still write their zeros)
+    // Straight from the accumulators: through LDS, whole rows at a time, took 3-9 % longer here (one workgroup per CU: nothing
+    // else runs meanwhile)
 #pragma unroll
     for (int wh = 0; wh < 2; ++wh)
 #pragma unroll
@@ -706,24 +769,43 @@ constexpr int kRows = 16;              // rows that fp8_rows_kernel can take
 constexpr size_t kRowsLds = 128 * 1024;   // its quantised rows in LDS
 constexpr int kCUs = 256;
 
-struct Plan { int kind, bm, bn, splits, per_split; };   // kind 0: fp8_rows_kernel, 1: fp8_gemm_kernel, 2: fp8_gemm8_kernel
+struct Plan { int kind, bm, bn, splits, per_split; long long body; };   // kind 0: fp8_rows_kernel, 1: fp8_gemm_kernel, 2: fp8_gemm8_kernel
 size_t rows_lds(long long M, int per_split) { return ((size_t)per_split * M * 129 + 15) & ~(size_t)15; }
 void set_splits(Plan& p, long long s, int kblocks) {
     if (s < 1) s = 1;
     p.per_split = (int)yfs_cdiv(kblocks, s);
     p.splits = (int)yfs_cdiv(kblocks, p.per_split);
 }
-// Operands that are both in 8 bits.
+// Operands that are both in 8 bits.  The largest tile of which there are enough for the chip (measured on the sizes in
+// brackets, us, against the next best):
+//   256 x 256 from two thirds of a round of 256 on, where they are three quarters full (3000 x 4096 x 4096: 49 / 56; 2048 x 4096 x 4096, half a round: 47 / 38)
+//   128 x 128 from two workgroups per CU on (2048 x 4096 x 4096: 38 / 50)
+//   64 x 128  from one per CU on (2048 x 2048 x 2048: 16 / 18; 64 x 50176 x 4096: 48 / 56)
+//   64 x 64   from three quarters of that on (300 x 4096 x 4096: 17 / 21)
+//   else 64 x 128 with the reduction split until there is one per CU, 4 blocks or more each (64 x 4096 x 50176: 44 / 47)
+// `exact` (fp32 outputs): no 256 x 256 form; 8 waves on the 128 x 128 tile where the reduction is so short that the stores
+// are what counts (4096 x 50176 x 64: 139 / 157; 4096 x 4096 x 4096: 126 / 116 the other way round).
 Plan plan_tiles(long long M, long long N, int kblocks, bool exact) {
-    Plan p = {1, 128, 128, 1, kblocks};
-    if (!exact && M > 128 && yfs_cdiv(M, 256) * yfs_cdiv(N, 256) >= kCUs && kblocks >= 4) {
+    Plan p = {1, 128, 128, 1, kblocks, 0};
+    const long long mt = yfs_cdiv(M, 256), nt = yfs_cdiv(N, 256), t256 = mt * nt;
+    if (!exact && 3 * t256 >= 2 * kCUs && 4 * M * N >= 3 * t256 * 65536) {
         p.kind = 2;
         p.bm = p.bn = 256;
+        // A last round of fewer than half the CUs costs as much as a full one: its tile rows go to the small tiles instead
+        const long long over = t256 % kCUs;
+        const long long whole = t256 > kCUs && over > 0 && over <= kCUs / 2 ? (t256 - over) / nt : mt;
+        p.body = whole * 256 < M ? whole * 256 : M;
         return p;
     }
-    if (M <= 64) p.bm = p.bn = 64;
-    const long long tiles = yfs_cdiv(M, p.bm) * yfs_cdiv(N, p.bn);
-    long long s = tiles >= kCUs ? 1 : 2 * kCUs / tiles;
+    if (yfs_cdiv(M, 128) * yfs_cdiv(N, 128) >= 2 * kCUs - kCUs / 4) return p;
+    p.bm = 64;
+    const long long wide = yfs_cdiv(M, 64) * yfs_cdiv(N, 128);
+    if (wide >= kCUs) return p;
+    if (yfs_cdiv(M, 64) * yfs_cdiv(N, 64) >= kCUs - kCUs / 4) {
+        p.bn = 64;
+        return p;
+    }
+    long long s = kCUs / wide;
     if (s > kblocks / 4) s = kblocks / 4;
     set_splits(p, s, kblocks);
     return p;
@@ -731,7 +813,7 @@ Plan plan_tiles(long long M, long long N, int kblocks, bool exact) {
 // x in its own type: few enough rows are quantised by the workgroups that multiply them.
 Plan plan_matmul(long long M, long long N, int kblocks, bool exact) {
     if (M <= kRows) {
-        Plan p = {0, 16, 16, 1, kblocks};
+        Plan p = {0, 16, 16, 1, kblocks, 0};
         const long long tiles = yfs_cdiv(N, 16);
         long long s = tiles >= kCUs ? 1 : kCUs / tiles;
         if (s > kblocks / 64) s = kblocks / 64;
@@ -759,9 +841,10 @@ int launch_tiles(const GemmArgs& g, hipStream_t s) {
     const dim3 grid((unsigned)yfs_cdiv(g.N, BN), (unsigned)yfs_cdiv(g.M, BM), (unsigned)g.splits);
     auto kern = fp8_gemm_kernel<FM, FN, WM, WN, S, ROWB, EXACT, TO>;
     // a short reduction leaves the rest of the ring to other workgroups
-    const int lds = STAGE * (g.per_split < S ? g.per_split : S);
-    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, STAGE * S);
-    YFS_REQUIRE(e == hipSuccess, YFS_ERR_LAUNCH, "fp8_gemm_kernel: cannot reserve %d bytes of LDS", STAGE * S);
+    constexpr int TILE_OUT = sizeof(TO) == 4 ? BM * (BN * 4 + 16) : 0, MOST = STAGE * S > TILE_OUT ? STAGE * S : TILE_OUT;
+    const int ring = STAGE * (g.per_split < S ? g.per_split : S), lds = ring > TILE_OUT ? ring : TILE_OUT;
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, MOST);
+    YFS_REQUIRE(e == hipSuccess, YFS_ERR_LAUNCH, "fp8_gemm_kernel: cannot reserve %d bytes of LDS", MOST);
     kern<<<grid, 64 * NW, lds, s>>>(g);
     YFS_CHECK_LAUNCH("fp8_gemm_kernel");
     yfs_note_kernel("fp8_gemm_kernel<%d,%d,splits%d>", BM, BN, g.splits);
@@ -775,22 +858,46 @@ int launch_gemm8(const GemmArgs& g, hipStream_t s) {
     YFS_REQUIRE(e == hipSuccess, YFS_ERR_LAUNCH, "fp8_gemm8_kernel: cannot reserve %d bytes of LDS", G8_LDS);
     kern<<<dim3((unsigned)(yfs_cdiv(g.M, 256) * yfs_cdiv(g.N, 256))), 512, G8_LDS, s>>>(g);
     YFS_CHECK_LAUNCH("fp8_gemm8_kernel");
-    yfs_note_kernel("fp8_gemm8_kernel");
     return YFS_OK;
 }
 
 template <bool ROWB, bool EXACT, typename TO>
 int gemm(GemmArgs g, hipStream_t s) {
-    const Plan p = plan_tiles(g.M, g.N, g.kblocks, EXACT || ROWB);
+    const Plan p = plan_tiles(g.M, g.N, g.kblocks, EXACT);
     g.splits = p.splits;
     g.per_split = p.per_split;
     g.groups_a = groups64(g.M);
     g.groups_b = groups64(g.N);
     if constexpr (!EXACT && !ROWB) {
-        if (p.kind == 2) return launch_gemm8<TO>(g, s);
+        if (p.kind == 2) {
+            // Whole rounds of 256 tiles by the large kernel; a few tile rows that would start another round by the small tiles
+            const long long rest = g.M - p.body;
+            if (rest > 0) {
+                GemmArgs r = g;
+                r.a += p.body * g.kblocks * 128;
+                r.row0 = p.body;
+                r.out = (TO*)g.out + p.body * g.N;
+                r.M = rest;
+                const bool wide = yfs_cdiv(rest, 64) * yfs_cdiv(g.N, 128) >= kCUs;
+                const int rc = wide ? launch_tiles<4, 2, 1, 4, 2, ROWB, EXACT, TO>(r, s) : launch_tiles<2, 2, 2, 2, 3, ROWB, EXACT, TO>(r, s);
+                if (rc != YFS_OK) return rc;
+                g.M = p.body;
+            }
+            const int rc = launch_gemm8<TO>(g, s);
+            if (rc == YFS_OK) yfs_note_kernel("fp8_gemm8_kernel<rest%lld>", rest);
+            return rc;
+        }
     }
-    if (p.bm == 64) return launch_tiles<2, 2, 2, 2, 4, ROWB, EXACT, TO>(g, s);
-    return launch_tiles<4, 4, 2, 2, 2, ROWB, EXACT, TO>(g, s);
+    if (p.bm == 128) {
+        if constexpr (EXACT) {
+            if (g.kblocks <= 4) return launch_tiles<4, 2, 2, 4, 2, ROWB, EXACT, TO>(g, s);
+        }
+        return launch_tiles<4, 4, 2, 2, 2, ROWB, EXACT, TO>(g, s);
+    }
+    if (p.bn == 64) return launch_tiles<2, 2, 2, 2, 3, ROWB, EXACT, TO>(g, s);
+    // (unsplit, four workgroups of two stages per CU; split, there is one per CU, and three stages keep more on their way)
+    if (p.splits == 1) return launch_tiles<4, 2, 1, 4, 2, ROWB, EXACT, TO>(g, s);
+    return launch_tiles<4, 2, 1, 4, 3, ROWB, EXACT, TO>(g, s);
 }
 
 template <typename T, typename TO>
@@ -832,8 +939,8 @@ YFS_API int yfs_fp8_quantize_weight(const void* w, int dtype, int64_t ld, int64_
     YFS_REQUIRE(known(dtype), YFS_ERR_UNSUPPORTED, "yfs_fp8_quantize_weight: unknown dtype %d", dtype);
     REQUIRE_ALIGNED("yfs_fp8_quantize_weight", q);
     REQUIRE_ALIGNED("yfs_fp8_quantize_weight", qt);
-    const QuantArgs g = {w, ld, N, K, (unsigned char*)q, (unsigned char*)scale, (unsigned char*)qt, (unsigned char*)scale_t, nullptr, 0, 0};
-    return qt ? quantize<true, true, true>(g, dtype, (hipStream_t)stream) : quantize<true, true, false>(g, dtype, (hipStream_t)stream);
+    const QuantArgs g = {w, ld, N, K, (unsigned char*)q, (unsigned char*)scale, (unsigned char*)qt, (unsigned char*)scale_t, nullptr, 0, 0, 0};
+    return qt ? quantize_blocks<true>(g, dtype, (hipStream_t)stream) : quantize_blocks<false>(g, dtype, (hipStream_t)stream);
 }
 
 YFS_API size_t yfs_fp8_packed_scale_bytes(int64_t rows, int64_t cols) {
@@ -849,11 +956,8 @@ YFS_API int yfs_fp8_quantize_rows(const void* x, int dtype, int64_t ld, int64_t 
     REQUIRE_ALIGNED("yfs_fp8_quantize_rows", q);
     REQUIRE_ALIGNED("yfs_fp8_quantize_rows", qt);
     const QuantArgs g = {x, ld, M, K, (unsigned char*)q, (unsigned char*)scale, (unsigned char*)qt, (unsigned char*)scale_t, colsum,
-                         groups64(M), groups64(K)};
-    hipStream_t s = (hipStream_t)stream;
-    if (q && qt) return quantize<false, true, true>(g, dtype, s);
-    if (q) return colsum ? quantize<false, true, false>(g, dtype, s) : quantize_rows_only(g, dtype, s);
-    return quantize<false, false, true>(g, dtype, s);
+                         groups64(M), groups64(K), 0};
+    return quantize_rows(g, dtype, (hipStream_t)stream);
 }
 
 // (whatever the output's type: the larger of the two forms)
@@ -868,7 +972,9 @@ YFS_API int yfs_fp8_gemm(const void* aq, const void* a_scale, const void* bq, co
     YFS_REQUIRE(aq && a_scale && bq && b_scale && out, YFS_ERR_INVALID_ARG, "yfs_fp8_gemm: null pointer");
     REQUIRE_SIZES("yfs_fp8_gemm", M, N, K);
     YFS_REQUIRE(known(out_dtype), YFS_ERR_UNSUPPORTED, "yfs_fp8_gemm: unknown dtype %d", out_dtype);
-    YFS_REQUIRE(!accumulate || out_dtype == YFS_F32, YFS_ERR_UNSUPPORTED, "yfs_fp8_gemm: only an fp32 output accumulates");
+    YFS_REQUIRE(!b_row_scales || out_dtype == YFS_F32, YFS_ERR_UNSUPPORTED, "yfs_fp8_gemm: row scales on both sides need an fp32 output");
+    YFS_REQUIRE(!accumulate || (out_dtype == YFS_F32 && slope == 1.0f), YFS_ERR_UNSUPPORTED,
+                "yfs_fp8_gemm: only an fp32 output without an activation accumulates");
     YFS_REQUIRE(slope >= 0.0f && slope <= 1.0f, YFS_ERR_INVALID_ARG, "yfs_fp8_gemm: slope %g not in [0, 1]", slope);
     REQUIRE_ALIGNED("yfs_fp8_gemm", aq);
     REQUIRE_ALIGNED("yfs_fp8_gemm", a_scale);
@@ -876,12 +982,9 @@ YFS_API int yfs_fp8_gemm(const void* aq, const void* a_scale, const void* bq, co
     const size_t need = yfs_fp8_gemm_workspace_bytes(M, N, K);
     YFS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), YFS_ERR_WORKSPACE, "yfs_fp8_gemm: workspace needs %zu bytes", need);
     GemmArgs g = {(const unsigned char*)aq, (const unsigned char*)a_scale, (const unsigned char*)bq, (const unsigned char*)b_scale, bias, out,
-                  (float*)workspace, M, N, (int)yfs_cdiv(K, 128), 1, 0, 0, 0, slope, accumulate};
+                  (float*)workspace, M, N, (int)yfs_cdiv(K, 128), 1, 0, 0, 0, 0, slope, accumulate};
     hipStream_t s = (hipStream_t)stream;
-    if (b_row_scales) {
-        if (out_dtype == YFS_F32) return gemm<true, true, float>(g, s);
-        return out_dtype == YFS_BF16 ? gemm<true, false, bf16_t>(g, s) : gemm<true, false, _Float16>(g, s);
-    }
+    if (b_row_scales) return gemm<true, true, float>(g, s);
     if (out_dtype == YFS_F32) return gemm<false, true, float>(g, s);
     return out_dtype == YFS_BF16 ? gemm<false, false, bf16_t>(g, s) : gemm<false, false, _Float16>(g, s);
 }
@@ -917,7 +1020,7 @@ YFS_API int yfs_fp8_matmul(const void* x, int x_dtype, int64_t ld, const void* w
     const Plan p = plan_matmul(M, N, (int)yfs_cdiv(K, 128), true);
     if (p.kind == 0) {
         const GemmArgs g = {nullptr, nullptr, (const unsigned char*)wq, (const unsigned char*)w_scale, bias, y, (float*)workspace,
-                            M, N, (int)yfs_cdiv(K, 128), 1, 0, 0, 0, slope, 0};
+                            M, N, (int)yfs_cdiv(K, 128), 1, 0, 0, 0, 0, slope, 0};
         hipStream_t s = (hipStream_t)stream;
         if (x_dtype == YFS_F32) return matmul_rows<float>(g, p, x, ld, K, out_dtype, s);
         if (x_dtype == YFS_BF16) return matmul_rows<bf16_t>(g, p, x, ld, K, out_dtype, s);
@@ -1047,11 +1150,12 @@ YFS_API int yfs_fp8_linear_bwd(const void* dy, int dy_dtype, int64_t lddy, void*
                 "yfs_fp8_linear_bwd: workspace needs %zu bytes, 256-byte aligned", f.bytes);
     YFS_REQUIRE(saved && saved_bytes >= k.bytes && aligned256(saved), YFS_ERR_WORKSPACE,
                 "yfs_fp8_linear_bwd: saved needs %zu bytes, 256-byte aligned", k.bytes);
-    int rc = yfs_fp8_quantize_rows(dy, dy_dtype, lddy, M, N, f.dq, f.ds, f.dqt, f.dst, f.colsum, stream);
+    const bool direct = db && M <= 128 && !accumulate_b;   // one tile of rows: its column sums are db
+    int rc = yfs_fp8_quantize_rows(dy, dy_dtype, lddy, M, N, f.dq, f.ds, f.dqt, f.dst, direct ? db : f.colsum, stream);
     if (rc == YFS_OK && dx)
         rc = yfs_fp8_gemm(f.dq, f.ds, k.wqt, k.wst, 0, nullptr, dx, dx_dtype, M, K, N, 1.0f, 0, f.part, f.part_bytes, stream);
     if (rc == YFS_OK && dw)
         rc = yfs_fp8_gemm(f.dqt, f.dst, k.xqt, k.xst, 1, nullptr, dw, YFS_F32, N, K, M, 1.0f, accumulate_w, f.part, f.part_bytes, stream);
-    if (rc == YFS_OK && db) rc = yfs_fp8_colsum(f.colsum, yfs_cdiv(M, 128), N, db, accumulate_b, stream);
+    if (rc == YFS_OK && db && !direct) rc = yfs_fp8_colsum(f.colsum, yfs_cdiv(M, 128), N, db, accumulate_b, stream);
     return rc;
 }
