@@ -110,11 +110,11 @@ def test_views_and_special_values(dtype):
 
 
 @pytest.mark.gpu
-def test_counter_is_the_element_index_past_32_bits():
-    """An fp16 tensor of 2^32 + 4096 elements (8 GiB): the last elements use counters of their own."""
+@pytest.mark.parametrize("n", [(1 << 32) + 4096, (1 << 34) + 4100])
+def test_counter_is_the_element_index_past_32_bits(n):
+    """fp16 tensors of 8 and 32 GiB: the last elements use counters of their own, of 33 bits in the second."""
     import yolo_from_scratch_amd as yfs
     from oracle.fc_ref import philox4x32_10
-    n = (1 << 32) + 4096
     x = torch.ones(n, device=DEV, dtype=torch.float16)
     y = yfs.dropout(x, 0.5, 31337)
     tail = 8192

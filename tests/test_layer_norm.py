@@ -254,6 +254,50 @@ def test_nothing_is_written_behind_the_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(9, 33), (5, 1030), (40, 2501), (3, 9001)])
+def test_library_on_rows_that_share_no_alignment(rows, cols, dtype):
+    """Odd widths through the library itself: rows at a stride of their own and a start at an odd element, forward and backward,
+    with guards behind every output."""
+    from yolo_from_scratch_amd import _lib as L
+    t = DTYPES[dtype]
+    x0, w, b, dy0 = _inputs(rows, cols, t)
+    big = torch.full((2, rows * (cols + 5) + 8), 2.0, device=DEV).to(t)
+    x, dy = [v[1:1 + rows * (cols + 5)].view(rows, cols + 5)[:, :cols] for v in big]
+    x.copy_(x0), dy.copy_(dy0)
+    y = torch.full((2, rows * cols + 64), 3.0, device=DEV).to(t)
+    stats, sums = torch.full((2, rows), 3.0, device=DEV), torch.full((2, cols + 8), 3.0, device=DEV)
+    lib, s, code = L.lib(), torch.cuda.current_stream().cuda_stream, L.DTYPES[t]
+    L.check(lib.yfs_layer_norm_fwd(x.data_ptr(), cols + 5, w.data_ptr(), b.data_ptr(), y[0].data_ptr(), stats[0].data_ptr(),
+                                   stats[1].data_ptr(), rows, cols, 1e-5, code, s), "fwd")
+    need = lib.yfs_layer_norm_bwd_workspace_bytes(rows, cols, code)
+    ws = torch.full((need + 64,), 7, device=DEV, dtype=torch.uint8)
+    dx = y[1, 1:]                                       # an odd start
+    L.check(lib.yfs_layer_norm_bwd(dy.data_ptr(), cols + 5, x.data_ptr(), cols + 5, w.data_ptr(), stats[0].data_ptr(),
+                                   stats[1].data_ptr(), dx.data_ptr(), sums[0].data_ptr(), sums[1].data_ptr(), rows, cols, code,
+                                   ws.data_ptr(), need, s), "bwd")
+    n = rows * cols
+    assert (y[0, n:] == 3).all() and (dx[n:] == 3).all() and (y[1, :1] == 3).all() and (sums[:, cols:] == 3).all() and (ws[need:] == 7).all()
+    _check_forward(_np(y[0, :n]).reshape(rows, cols), _np(x0), _np(w), _np(b), 1e-5, t)
+    _check_backward(_np(dx[:n]).reshape(rows, cols), _np(sums[0, :cols]), _np(sums[1, :cols]), _np(dy0), _np(x0), _np(w), 1e-5, t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,dtype", [(9001, 257, "bf16"), (5003, 1470, "f16"), (4100, 3001, "bf16"), (3000, 1471, "f32"),
+                                             (20003, 9, "bf16"), (2500, 8193, "bf16")])
+def test_odd_widths_with_many_rows(rows, cols, dtype):
+    """Column sums in the pass of dx, over rows that begin at every place of an aligned 16 bytes."""
+    import yolo_from_scratch_amd as yfs
+    x, w, b, dy = _inputs(rows, cols, DTYPES[dtype])
+    for v in (x, w, b):
+        v.requires_grad_()
+    y = yfs.layer_norm(x, w, b)
+    got = torch.autograd.grad(y, (x, w, b), dy)
+    _check_forward(_np(y), _np(x), _np(w), _np(b), 1e-5, x.dtype)
+    _check_backward(*[_np(v) for v in got], _np(dy), _np(x), _np(w), 1e-5, x.dtype)
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """<dx, v> against (f(x + sv) - f(x - sv)) / 2s in fp32.  With s = 2^-6 and |v| = 1 a component's rounding enters as
     2^-24 |y| / s = 2^-18 |y dy| (random signs over 4000 terms), the third derivative as s^2 / 6 of order one: 1e-3 of the

@@ -34,8 +34,8 @@ __global__ void __launch_bounds__(kThreads) fc_epilogue_fwd_kernel(const float* 
         unsigned r[8];
         if (p_drop > 0.0f) {
             unsigned r0[4], r1[4];
-            yfs_philox4(seed, (unsigned long long)id * 2, r0);
-            yfs_philox4(seed, (unsigned long long)id * 2 + 1, r1);
+            yfs_philox4(seed, (unsigned)(id * 2), (unsigned)((unsigned long long)(id * 2) >> 32), r0);
+            yfs_philox4(seed, (unsigned)(id * 2 + 1), (unsigned)((unsigned long long)(id * 2) >> 32), r1);
 #pragma unroll
             for (int j = 0; j < 4; ++j) { r[j] = r0[j]; r[4 + j] = r1[j]; }
         }

@@ -31,9 +31,11 @@ __device__ __forceinline__ float2 row_sum(float a, float b, int G, float2* red, 
     return make_float2(a, b);
 }
 
-// One group of G threads per row (BLOCK: the workgroup), NV vectors of VE elements per thread.
-template <typename T, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_fwd_kernel(const T* __restrict__ x, long long xs, const float* __restrict__ w,
+// One group of G threads per row (BLOCK: the workgroup), NV vectors of VE elements per thread.  ODD: the width is no multiple of
+// VE, and the row's last vector is cut off.  The workgroups stay, 16 waves a CU, with weight and bias in their registers (12544 x
+// 4096 bf16: 35 us, 5.9 TB/s; one workgroup per row 43; reading weight and bias again for every row 44).
+template <typename T, int NV, bool BLOCK, bool ODD>
+__global__ void __launch_bounds__(BLOCK ? 512 : 256) ln_fwd_kernel(const T* __restrict__ x, long long xs, const float* __restrict__ w,
                                                                    const float* __restrict__ b, T* __restrict__ y,
                                                                    float* __restrict__ mean, float* __restrict__ rstd,
                                                                    long long rows, int cols, float eps, int lg) {
@@ -42,26 +44,53 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_fwd_kernel(const T* __r
     const int G = BLOCK ? (int)blockDim.x : 1 << lg;
     const int t = BLOCK ? (int)threadIdx.x : (int)threadIdx.x & (G - 1);
     const long long rpb = BLOCK ? 1 : 256 >> lg;
+    const long long first = (long long)blockIdx.x * rpb + (BLOCK ? 0 : (int)threadIdx.x >> lg), stride = (long long)gridDim.x * rpb;
+    bool whole[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) whole[i] = ODD && __all((i * G + t + 1) * VE <= cols);
     const float inv = 1.0f / (float)cols;
-    for (long long row = (long long)blockIdx.x * rpb + (BLOCK ? 0 : (int)threadIdx.x >> lg); row < rows; row += (long long)gridDim.x * rpb) {
+    // weight and bias stay in registers where there is room for them
+    constexpr bool KEEP = NV <= 3;
+    float wv[KEEP ? NV : 1][VE], bv[KEEP ? NV : 1][VE];
+    auto params = [&](int i, float (&pw)[VE], float (&pb)[VE]) {
+        const int c = (i * G + t) * VE;
+        load_vec_or(w, c, cols, pw, 1.0f);
+        load_vec_or(b, c, cols, pb, 0.0f);
+    };
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) params(i, wv[i], bv[i]);
+    }
+    T ahead[NV][VE];
+    auto fetch = [&](long long row) {   // the next row is on its way while one is reduced
+#pragma unroll
+        for (int i = 0; i < NV; ++i) load_row<ODD>(x + row * xs, (i * G + t) * VE, cols, whole[i], ahead[i]);
+    };
+    if (first < rows) fetch(first);
+    for (long long row = first; row < rows; row += stride) {
         float v[NV][VE];
         float s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + t) * VE;
-            load_vec(x + row * xs + c, cols - c, v[i]);
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < VE; ++j) s += v[i][j];
-        }
+            for (int j = 0; j < VE; ++j) {
+                v[i][j] = (float)ahead[i][j];
+                s += v[i][j];
+            }
+        if (row + stride < rows) fetch(row + stride);
         const float mu = row_sum<BLOCK>(s, 0.0f, G, red, 0).x * inv;
         float q = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int n = cols - (i * G + t) * VE;
+            const int c = (i * G + t) * VE;
+            if (!(ODD && whole[i])) {   // (what lies behind the row counts as its mean)
+#pragma unroll
+                for (int j = 0; j < VE; ++j) v[i][j] = (ODD ? c + j < cols : c < cols) ? v[i][j] : mu;
+            }
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
                 v[i][j] -= mu;
-                q += j < n ? v[i][j] * v[i][j] : 0.0f;
+                q += v[i][j] * v[i][j];
             }
         }
         const float r = 1.0f / sqrtf(row_sum<BLOCK>(q, 0.0f, G, red, 1).x * inv + eps);
@@ -71,13 +100,11 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_fwd_kernel(const T* __r
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + t) * VE;
-            float wv[VE], bv[VE];
-            load_vec_or(w, c, cols - c, wv, 1.0f);
-            load_vec_or(b, c, cols - c, bv, 0.0f);
+            const int k = KEEP ? i : 0;
+            if constexpr (!KEEP) params(i, wv[0], bv[0]);
 #pragma unroll
-            for (int j = 0; j < VE; ++j) v[i][j] = v[i][j] * r * wv[j] + bv[j];
-            store_vec(y + row * cols + c, cols - c, v[i]);
+            for (int j = 0; j < VE; ++j) v[i][j] = v[i][j] * r * wv[k][j] + bv[k][j];
+            store_row<ODD>(y + row * cols, (i * G + t) * VE, cols, whole[i], v[i]);
         }
     }
 }
@@ -112,8 +139,8 @@ __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(const T* __restrict__
         for (long long c = (long long)threadIdx.x * VE; c < cols; c += 1024 * VE) {
             float wv[VE], bv[VE];
             load_vec(xr + c, cols - c, v);
-            load_vec_or(w, c, cols - c, wv, 1.0f);
-            load_vec_or(b, c, cols - c, bv, 0.0f);
+            load_vec_or(w, c, cols, wv, 1.0f);
+            load_vec_or(b, c, cols, bv, 0.0f);
 #pragma unroll
             for (int j = 0; j < VE; ++j) v[j] = (v[j] - mu) * r * wv[j] + bv[j];
             store_vec(y + row * cols + c, cols - c, v);
@@ -182,10 +209,10 @@ __device__ __forceinline__ void column_sums(const BwdArgs& g, int block, float* 
 }
 
 // dx by rows as in the forward pass.  ACC: the thread that holds a column of dx sums its dw and db too, over the rows that its
-// workgroup meets: x and dy are read once for all three.  That needs many rows per workgroup, or the partial sums outgrow them
-// (200704 x 256 bf16: 53 + 114 us as two kernels); for few rows the column sums are other workgroups of the same launch.
-template <typename T, int NV, bool BLOCK, bool ACC>
-__global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_bwd_kernel(BwdArgs g) {
+// workgroup meets: x and dy are read once for all three (200704 x 256 bf16: 55 us, 5.6 TB/s; 53 + 114 as two kernels).  That needs
+// many rows per workgroup, or the partial sums outgrow them; for few rows the column sums are other workgroups of the same launch.
+template <typename T, int NV, bool BLOCK, bool ACC, bool ODD>
+__global__ void __launch_bounds__(BLOCK ? 512 : 256) ln_bwd_kernel(BwdArgs g) {
     constexpr int VE = 16 / sizeof(T);
     __shared__ float2 red[32];
     extern __shared__ float sums[];
@@ -196,29 +223,42 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_bwd_kernel(BwdArgs g) {
     const int G = BLOCK ? (int)blockDim.x : 1 << g.lg;
     const int t = BLOCK ? (int)threadIdx.x : (int)threadIdx.x & (G - 1);
     const long long rpb = BLOCK ? 1 : 256 >> g.lg;
+    const long long first = (long long)blockIdx.x * rpb + (BLOCK ? 0 : (int)threadIdx.x >> g.lg), stride = (long long)g.dx_blocks * rpb;
+    bool whole[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) whole[i] = ODD && __all((i * G + t + 1) * VE <= g.cols);
     const float inv = 1.0f / (float)g.cols;
     float wv[NV][VE], aw[ACC ? NV : 1][VE], ab[ACC ? NV : 1][VE];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (i * G + t) * VE;
-        load_vec_or(g.w, c, g.cols - c, wv[i], 1.0f);
+        load_vec_or(g.w, (i * G + t) * VE, g.cols, wv[i], 1.0f);
         if (ACC) {
 #pragma unroll
             for (int j = 0; j < VE; ++j) aw[i][j] = ab[i][j] = 0.0f;
         }
     }
     int slot = 0;
-    for (long long row = (long long)blockIdx.x * rpb + (BLOCK ? 0 : (int)threadIdx.x >> g.lg); row < g.rows; row += (long long)g.dx_blocks * rpb) {
+    for (long long row = first; row < g.rows; row += stride) {   // (with the next row ahead, as in the forward pass, 200704 x 256 bf16 takes 75 us for 55)
         const float mu = g.mean[row], r = g.rstd[row];
         float h[NV][VE], d[NV][VE], s1 = 0.0f, s2 = 0.0f;
+        T xr[NV][VE], dr[NV][VE];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + t) * VE, n = g.cols - c;
-            load_vec((const T*)g.x + row * g.xs + c, n, h[i]);
-            load_vec((const T*)g.dy + row * g.dys + c, n, d[i]);
+            load_row<ODD>((const T*)g.x + row * g.xs, (i * G + t) * VE, g.cols, whole[i], xr[i]);
+            load_row<ODD>((const T*)g.dy + row * g.dys, (i * G + t) * VE, g.cols, whole[i], dr[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * G + t) * VE;
+#pragma unroll
+            for (int j = 0; j < VE; ++j) h[i][j] = ((float)xr[i][j] - mu) * r;
+            if (!(ODD && whole[i])) {
+#pragma unroll
+                for (int j = 0; j < VE; ++j) h[i][j] = (ODD ? c + j < g.cols : c < g.cols) ? h[i][j] : 0.0f;
+            }
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
-                h[i][j] = j < n ? (h[i][j] - mu) * r : 0.0f;
+                d[i][j] = (float)dr[i][j];
                 if (ACC) {
                     aw[i][j] += d[i][j] * h[i][j];
                     ab[i][j] += d[i][j];
@@ -233,10 +273,9 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_bwd_kernel(BwdArgs g) {
         const float m1 = s.x * inv, m2 = s.y * inv;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + t) * VE;
 #pragma unroll
             for (int j = 0; j < VE; ++j) d[i][j] = r * (d[i][j] - m1 - h[i][j] * m2);
-            store_vec((T*)g.dx + row * g.cols + c, g.cols - c, d[i]);
+            store_row<ODD>((T*)g.dx + row * g.cols, (i * G + t) * VE, g.cols, whole[i], d[i]);
         }
     }
     if constexpr (ACC && BLOCK) {
@@ -247,19 +286,21 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_bwd_kernel(BwdArgs g) {
             store_vec(g.db + (long long)blockIdx.x * 2 * g.cols + c, g.cols - c, ab[i]);
         }
     } else if constexpr (ACC) {
-        const int grp = (int)threadIdx.x >> g.lg, groups = 256 >> g.lg, width = G * NV * VE;
+        const int grp = (int)threadIdx.x >> g.lg, groups = 256 >> g.lg;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
-                sums[(grp * 2 + 0) * width + (i * G + t) * VE + j] = aw[i][j];
-                sums[(grp * 2 + 1) * width + (i * G + t) * VE + j] = ab[i][j];
+                const int c = (i * G + t) * VE + j;
+                if (c < g.cols) {
+                    sums[(grp * 2 + 0) * g.cols + c] = aw[i][j];
+                    sums[(grp * 2 + 1) * g.cols + c] = ab[i][j];
+                }
             }
         __syncthreads();
         for (int k = threadIdx.x; k < 2 * g.cols; k += 256) {
-            const int which = k >= g.cols, c = k - which * g.cols;
             float v = 0.0f;
-            for (int q = 0; q < groups; ++q) v += sums[(q * 2 + which) * width + c];
+            for (int q = 0; q < groups; ++q) v += sums[q * 2 * g.cols + k];
             g.dw[(long long)blockIdx.x * 2 * g.cols + k] = v;   // (db lies cols behind dw)
         }
     }
@@ -284,7 +325,7 @@ __global__ void __launch_bounds__(1024) ln_bwd_long_kernel(BwdArgs g) {
             const long long n = g.cols - c;
             load_vec(xr + c, n, h);
             load_vec(dr + c, n, d);
-            load_vec_or(g.w, c, n, wv, 1.0f);
+            load_vec_or(g.w, c, g.cols, wv, 1.0f);
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
                 s1 += d[j] * wv[j];
@@ -298,7 +339,7 @@ __global__ void __launch_bounds__(1024) ln_bwd_long_kernel(BwdArgs g) {
             const long long n = g.cols - c;
             load_vec(xr + c, n, h);
             load_vec(dr + c, n, d);
-            load_vec_or(g.w, c, n, wv, 1.0f);
+            load_vec_or(g.w, c, g.cols, wv, 1.0f);
 #pragma unroll
             for (int j = 0; j < VE; ++j) d[j] = r * (d[j] * wv[j] - m1 - (h[j] - mu) * r * m2);
             store_vec((T*)g.dx + row * g.cols + c, n, d);
@@ -327,21 +368,25 @@ __global__ void __launch_bounds__(1024) ln_reduce_kernel(const float* __restrict
     }
 }
 
-struct Shape { int nv, lg, threads; };   // threads > 256 or lg < 0: one workgroup per row; nv == 0: the long form
-Shape ln_shape(int cols, int esize, int max_nv_block) {
+constexpr int kCUs = 256;
+struct Shape { int nv, lg, threads; };   // lg >= 0: groups of 2^lg lanes; lg < 0: one workgroup per row; nv == 0: the long form
+// A wave per row up to `wave_most` vectors a lane (three, with dw and db summed, are 186 registers: 1470 bf16 columns 160 us against
+// 126 in workgroups of 128, 50000 rows backward; without sums three fit: 74 against 85 forward).  Longer rows have two vectors per
+// thread (4096 bf16 columns: 43 us against 49 with one, 12544 rows forward), up to `most` in a workgroup of 512.
+Shape ln_shape(int cols, int esize, int wave_most, int most) {
     const long long vecs = yfs_cdiv(cols, 16 / esize);
     for (int lg = 3; lg <= 6; ++lg)
         if (vecs <= (1 << lg)) return {1, lg, 256};
-    if (vecs <= 128) return {2, 6, 256};
-    for (int th = 256; th <= 1024; th *= 2)
-        if (vecs <= th) return {1, -1, th};
-    for (int nv = 2; nv <= max_nv_block; nv *= 2)
-        if (vecs <= 1024LL * nv) return {nv, -1, 1024};
+    for (int nv = 2; nv <= wave_most; ++nv)
+        if (vecs <= 64 * nv) return {nv, 6, 256};
+    for (int nv = 2; nv <= most; nv *= 2)
+        if (vecs <= 512LL * nv) return {nv, -1, (int)(yfs_cdiv(vecs, 64 * nv) * 64)};
     return {0, -1, 1024};
 }
+// Workgroups that take the rows in turn: 32 waves a CU where a wave has a row, 16 where a workgroup has one
 unsigned row_blocks(long long rows, const Shape& s) {
-    const long long nb = s.lg >= 0 ? yfs_cdiv(rows, 256 >> s.lg) : rows;
-    return (unsigned)(nb < 8192 ? nb : 8192);
+    const long long nb = s.lg >= 0 ? yfs_cdiv(rows, 256 >> s.lg) : rows, most = kCUs * (s.lg >= 0 ? 32 : 16) * 64 / s.threads;
+    return (unsigned)(nb < most ? nb : most);
 }
 
 // How the backward pass goes over the chip.  acc: dx and the column sums by the same workgroups, one partial sum each; else
@@ -349,12 +394,12 @@ unsigned row_blocks(long long rows, const Shape& s) {
 struct BwdPlan { Shape sh; bool acc; int dx_blocks, strips, parts; long long part_rows; };
 BwdPlan bwd_plan(long long rows, int cols, int esize, bool need_dx) {
     BwdPlan p;
-    p.sh = ln_shape(cols, esize, esize == 2 ? 2 : 4);
+    p.sh = ln_shape(cols, esize, 2, 4);
     p.dx_blocks = need_dx ? (int)row_blocks(rows, p.sh) : 0;
     p.strips = (int)yfs_cdiv(cols, 32 * (16 / esize));
     const long long rpb = p.sh.lg >= 0 ? 256 >> p.sh.lg : 1;
     // a partial sum is 8 bytes a column, a row of x, dy and dx 6 or 12: from 8 rows a workgroup on it is small next to them
-    const long long fill = p.sh.threads == 256 ? 1024 : (p.sh.threads == 512 ? 512 : 256);
+    const long long fill = kCUs * 16 * 64 / p.sh.threads;   // 16 waves per CU
     p.acc = need_dx && p.sh.nv > 0 && p.sh.nv <= 2 && rows >= fill / 2 * rpb * 8;
     if (p.acc) {
         const long long nb = rows / (rpb * 8);
@@ -375,19 +420,24 @@ BwdPlan bwd_plan(long long rows, int cols, int esize, bool need_dx) {
 template <typename T>
 int fwd(const void* x, long long xs, const float* w, const float* b, void* y, float* mean, float* rstd, long long rows, int cols,
         float eps, hipStream_t s) {
-    const Shape sh = ln_shape(cols, sizeof(T), sizeof(T) == 2 ? 4 : 8);
+    const bool odd = cols % (16 / (int)sizeof(T)) != 0;
+    const Shape sh = ln_shape(cols, sizeof(T), 3, sizeof(T) == 2 ? 4 : 8);
     const dim3 grid(row_blocks(rows, sh)), blk(sh.threads);
-#define LN_FWD(NV, BLOCK) ln_fwd_kernel<T, NV, BLOCK><<<grid, blk, 0, s>>>((const T*)x, xs, w, b, (T*)y, mean, rstd, rows, cols, eps, sh.lg)
+#define LN_FWD(NV, BLOCK)                                                                                                              \
+    do {                                                                                                                               \
+        if (odd) ln_fwd_kernel<T, NV, BLOCK, true><<<grid, blk, 0, s>>>((const T*)x, xs, w, b, (T*)y, mean, rstd, rows, cols, eps, sh.lg);   \
+        else ln_fwd_kernel<T, NV, BLOCK, false><<<grid, blk, 0, s>>>((const T*)x, xs, w, b, (T*)y, mean, rstd, rows, cols, eps, sh.lg);       \
+    } while (0)
     if (sh.nv == 0)
         ln_fwd_long_kernel<T><<<grid, blk, 0, s>>>((const T*)x, xs, w, b, (T*)y, mean, rstd, rows, cols, eps);
     else if (sh.lg >= 0) {
-        if (sh.nv == 1) LN_FWD(1, false); else LN_FWD(2, false);
-    } else switch (sh.nv) {
-        case 1: LN_FWD(1, true); break;
-        case 2: LN_FWD(2, true); break;
-        case 4: LN_FWD(4, true); break;
-        default:
-            if constexpr (sizeof(T) == 4) LN_FWD(8, true);
+        if (sh.nv == 1) LN_FWD(1, false);
+        else if (sh.nv == 2) LN_FWD(2, false);
+        else LN_FWD(3, false);
+    } else if (sh.nv == 2) LN_FWD(2, true);
+    else if (sh.nv == 4) LN_FWD(4, true);
+    else {
+        if constexpr (sizeof(T) == 4) LN_FWD(8, true);
     }
 #undef LN_FWD
     YFS_CHECK_LAUNCH("ln_fwd_kernel");
@@ -396,7 +446,7 @@ int fwd(const void* x, long long xs, const float* w, const float* b, void* y, fl
 
 template <typename T>
 int bwd(BwdArgs g, float* part, hipStream_t s) {
-    const bool sums = g.dw || g.db;
+    const bool sums = g.dw || g.db, odd = g.cols % (16 / (int)sizeof(T)) != 0;
     BwdPlan p = bwd_plan(g.rows, g.cols, sizeof(T), g.dx != nullptr);
     if (!sums) {
         p.acc = false;
@@ -416,18 +466,19 @@ int bwd(BwdArgs g, float* part, hipStream_t s) {
     if (!sums && !g.dx) return YFS_OK;
     const dim3 grid((unsigned)(p.dx_blocks + (p.acc ? 0 : (long long)p.strips * p.parts))), blk(p.sh.threads);
     // sums of the groups of a workgroup, or of the waves of a column strip
-    const size_t lds = p.acc ? (p.sh.lg >= 0 ? 512 * sizeof(float) * p.sh.nv * (16 / sizeof(T)) : 0)
+    const size_t lds = p.acc ? (p.sh.lg >= 0 ? (size_t)(256 >> p.sh.lg) * 2 * g.cols * sizeof(float) : 0)
                              : (sums ? (size_t)p.sh.threads / 64 * 2 * 32 * (16 / sizeof(T)) * sizeof(float) : 0);
-#define LN_BWD(NV, BLOCK) \
-    do { if (p.acc) ln_bwd_kernel<T, NV, BLOCK, true><<<grid, blk, lds, s>>>(g); else ln_bwd_kernel<T, NV, BLOCK, false><<<grid, blk, lds, s>>>(g); } while (0)
+#define LN_BWD(NV, BLOCK, ACC) \
+    do { if (odd) ln_bwd_kernel<T, NV, BLOCK, ACC, true><<<grid, blk, lds, s>>>(g); else ln_bwd_kernel<T, NV, BLOCK, ACC, false><<<grid, blk, lds, s>>>(g); } while (0)
     if (p.sh.nv == 0) ln_bwd_long_kernel<T><<<grid, blk, lds, s>>>(g);
     else if (p.sh.lg >= 0) {
-        if (p.sh.nv == 1) LN_BWD(1, false); else LN_BWD(2, false);
-    } else if (p.sh.nv == 1) LN_BWD(1, true);
-    else if (p.sh.nv == 2) LN_BWD(2, true);
-    else {
-        if constexpr (sizeof(T) == 4) ln_bwd_kernel<T, 4, true, false><<<grid, blk, lds, s>>>(g);
-    }
+        if (p.sh.nv == 1 && p.acc) LN_BWD(1, false, true);
+        else if (p.sh.nv == 1) LN_BWD(1, false, false);
+        else if (p.acc) LN_BWD(2, false, true);
+        else LN_BWD(2, false, false);
+    } else if (p.sh.nv == 4) LN_BWD(4, true, false);
+    else if (p.acc) LN_BWD(2, true, true);
+    else LN_BWD(2, true, false);
 #undef LN_BWD
     YFS_CHECK_LAUNCH("ln_bwd_kernel");
     if (sums && join) {

@@ -85,9 +85,9 @@ void once(const char* what) {
 
 // ---- layer norm ------------------------------------------------------------------------------------------------------
 Tensor ln_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, Tensor* stats) {
+    const c10::DeviceGuard guard(x.device());
     const Rows r(x);
     const Tensor w = f32_vector(weight), b = f32_vector(bias);
-    const c10::DeviceGuard guard(x.device());
     Tensor y = at::empty(x.sizes(), x.options());
     if (stats) *stats = at::empty({2, r.rows}, x.options().dtype(at::kFloat));
     if (r.rows) {
@@ -118,9 +118,9 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
         const int64_t bias_type = ctx->saved_data["bias"].toInt();
         const bool need_w = weight.defined() && ctx->needs_input_grad(1);
         const bool need_b = bias_type >= 0 && ctx->needs_input_grad(weight.defined() ? 2 : 1);
+        const c10::DeviceGuard guard(x.device());
         const Rows r(x), d(grads[0].scalar_type() == x.scalar_type() ? grads[0] : grads[0].to(x.scalar_type()));
         const Tensor w = f32_vector(weight);
-        const c10::DeviceGuard guard(x.device());
         const auto f = x.options().dtype(at::kFloat);
         Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : Tensor();
         Tensor dw = need_w ? (r.rows ? at::empty({r.cols}, f) : at::zeros({r.cols}, f)) : Tensor();

@@ -42,23 +42,29 @@ __device__ __forceinline__ float yfs_wave_sum(float v) {
     return v;   // lane 0 holds the sum, fixed reduction tree => deterministic
 }
 
-// Philox4x32-10 (Salmon et al., SC'11): counter = (element group, 0, 0, 0), key = seed.
+// Philox4x32-10 (Salmon et al., SC'11): counter = (element group, 0, 0, 0), key = seed.  Products are one 32 x 32 -> 64 bit
+// multiply-add each, the two exclusive-ors one three-operand instruction.
+__device__ __forceinline__ unsigned yfs_xor3(unsigned a, unsigned b, unsigned c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
 __device__ __forceinline__ void yfs_philox_round(unsigned (&c)[4], unsigned k0, unsigned k1) {
     const unsigned long long p0 = 0xD2511F53ull * c[0], p1 = 0xCD9E8D57ull * c[2];
     const unsigned h0 = (unsigned)(p0 >> 32), l0 = (unsigned)p0, h1 = (unsigned)(p1 >> 32), l1 = (unsigned)p1;
-    c[0] = h1 ^ c[1] ^ k0;
+    c[0] = yfs_xor3(h1, c[1], k0);
     c[1] = l1;
-    c[2] = h0 ^ c[3] ^ k1;
+    c[2] = yfs_xor3(h0, c[3], k1);
     c[3] = l0;
 }
-__device__ __forceinline__ void yfs_philox4(unsigned long long seed, unsigned long long ctr, unsigned (&out)[4]) {
-    unsigned c[4] = {(unsigned)ctr, (unsigned)(ctr >> 32), 0u, 0u};
+// ctr_hi: the counter's high word.  Where it is the same in a whole wave the first product of the second round is too, and
+// runs on the scalar unit.
+__device__ __forceinline__ void yfs_philox4(unsigned long long seed, unsigned ctr, unsigned ctr_hi, unsigned (&out)[4]) {
     unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
+    // round 1 by hand: its third and fourth words are zeros
+    const unsigned long long p0 = 0xD2511F53ull * ctr;
+    unsigned c[4] = {ctr_hi ^ k0, 0u, (unsigned)(p0 >> 32) ^ k1, (unsigned)p0};
 #pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        yfs_philox_round(c, k0, k1);
+    for (int r = 1; r < 10; ++r) {
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
+        yfs_philox_round(c, k0, k1);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = c[i];

@@ -17,6 +17,31 @@ __device__ __forceinline__ void load_vec(const T* p, long long n, float (&v)[VE]
     }
 }
 
+// The elements c .. c + VE - 1 of a row of n.  ODD false: n is a multiple of VE.  ODD true: `whole` says that the vectors of all lanes
+// of the wave lie inside the row, so that the one that crosses its end costs the others nothing.
+template <bool ODD, typename T, int VE = 16 / (int)sizeof(T)>
+__device__ __forceinline__ void load_row(const T* row, int c, int n, bool whole, T (&t)[VE]) {
+    if (ODD && whole) __builtin_memcpy(t, row + c, 16);
+    else if (ODD ? c + VE <= n : c < n) __builtin_memcpy(t, row + c, 16);
+    else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) t[j] = ODD && c + j < n ? row[c + j] : (T)0.0f;
+    }
+}
+template <bool ODD, typename T, int VE>
+__device__ __forceinline__ void store_row(T* row, int c, int n, bool whole, const float (&v)[VE]) {
+    T t[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) t[j] = (T)v[j];
+    if (ODD && whole) __builtin_memcpy(row + c, t, 16);
+    else if (ODD ? c + VE <= n : c < n) __builtin_memcpy(row + c, t, 16);
+    else if (ODD) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+            if (c + j < n) row[c + j] = t[j];
+    }
+}
+
 template <typename T, int VE>
 __device__ __forceinline__ void store_vec(T* p, long long n, const float (&v)[VE]) {
     if (n >= VE) {
@@ -31,17 +56,17 @@ __device__ __forceinline__ void store_vec(T* p, long long n, const float (&v)[VE
     }
 }
 
-// VE fp32 values (16-byte loads), or `none` where there is no tensor
+// VE fp32 values at c .. of n, or `none` where there is no tensor
 template <int VE>
 __device__ __forceinline__ void load_vec_or(const float* p, long long c, long long n, float (&v)[VE], float none) {
     if (!p) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) v[j] = none;
-    } else if (n >= VE) {
+    } else if (c + VE <= n) {
         __builtin_memcpy(v, p + c, VE * 4);
     } else {
 #pragma unroll
-        for (int j = 0; j < VE; ++j) v[j] = j < n ? p[c + j] : 0.0f;
+        for (int j = 0; j < VE; ++j) v[j] = c + j < n ? p[c + j] : 0.0f;
     }
 }
 
