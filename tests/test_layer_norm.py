@@ -284,9 +284,11 @@ def test_library_on_rows_that_share_no_alignment(rows, cols, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,cols,dtype", [(9001, 257, "bf16"), (5003, 1470, "f16"), (4100, 3001, "bf16"), (3000, 1471, "f32"),
-                                             (20003, 9, "bf16"), (2500, 8193, "bf16")])
-def test_odd_widths_with_many_rows(rows, cols, dtype):
-    """Column sums in the pass of dx, over rows that begin at every place of an aligned 16 bytes."""
+                                             (20003, 9, "bf16"), (2500, 8193, "bf16"), (1500, 4096, "f16"), (1200, 1536, "bf16"),
+                                             (9000, 96, "f32"), (1100, 8192, "f32")])
+def test_column_sums_of_many_rows(rows, cols, dtype):
+    """Column sums in the pass of dx, with a wave and with a workgroup per row, over rows that begin at every place of an aligned
+    16 bytes and over whole ones."""
     import yolo_from_scratch_amd as yfs
     x, w, b, dy = _inputs(rows, cols, DTYPES[dtype])
     for v in (x, w, b):

@@ -398,11 +398,11 @@ BwdPlan bwd_plan(long long rows, int cols, int esize, bool need_dx) {
     p.dx_blocks = need_dx ? (int)row_blocks(rows, p.sh) : 0;
     p.strips = (int)yfs_cdiv(cols, 32 * (16 / esize));
     const long long rpb = p.sh.lg >= 0 ? 256 >> p.sh.lg : 1;
-    // a partial sum is 8 bytes a column, a row of x, dy and dx 6 or 12: from 8 rows a workgroup on it is small next to them
-    const long long fill = kCUs * 16 * 64 / p.sh.threads;   // 16 waves per CU
-    p.acc = need_dx && p.sh.nv > 0 && p.sh.nv <= 2 && rows >= fill / 2 * rpb * 8;
+    // a partial sum is 8 bytes a column, written and read, a row of x, dy and dx 6 or 12: from 4 rows a workgroup on it is less than
+    // reading x and dy again
+    const long long fill = kCUs * 16 * 64 / p.sh.threads, nb = rows / (rpb * 4);   // 16 waves per CU
+    p.acc = need_dx && p.sh.nv > 0 && p.sh.nv <= 2 && nb >= kCUs;
     if (p.acc) {
-        const long long nb = rows / (rpb * 8);
         p.dx_blocks = (int)(nb < fill ? nb : fill);
         p.parts = p.dx_blocks;
         p.part_rows = 0;

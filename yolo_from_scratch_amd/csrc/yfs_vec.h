@@ -48,7 +48,7 @@ __device__ __forceinline__ void store_vec(T* p, long long n, const float (&v)[VE
         T t[VE];
 #pragma unroll
         for (int j = 0; j < VE; ++j) t[j] = (T)v[j];
-        __builtin_memcpy(p, t, 16);
+        __builtin_memcpy(p, t, VE * sizeof(T));
     } else {
 #pragma unroll
         for (int j = 0; j < VE; ++j)
