@@ -86,7 +86,9 @@ def binding():
             raise YfsError(f"yolo_from_scratch_amd/_binding.so cannot be loaded ({e}): build it with "
                            f"`make -C {os.path.join(_HERE, 'csrc')}`. There is no CPU fallback.") from e
         names = ("yfs_last_error", "yfs_layer_norm_fwd", "yfs_layer_norm_bwd", "yfs_layer_norm_bwd_workspace_bytes",
-                 "yfs_dropout_fwd", "yfs_dropout_bwd", "yfs_fp8_matmul", "yfs_fp8_matmul_workspace_bytes")
+                 "yfs_dropout_fwd", "yfs_dropout_bwd", "yfs_fp8_matmul", "yfs_fp8_matmul_workspace_bytes", "yfs_fp8_linear_saved_bytes",
+                 "yfs_fp8_linear_fwd_workspace_bytes", "yfs_fp8_linear_bwd_workspace_bytes", "yfs_fp8_linear_fwd",
+                 "yfs_fp8_linear_bwd")
         module.init({n: ctypes.cast(getattr(lib(), n), ctypes.c_void_p).value for n in names}, YfsError)
         _binding = module
     return _binding

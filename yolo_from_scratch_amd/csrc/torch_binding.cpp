@@ -1,4 +1,4 @@
-// Tensor side of the head operators whose calls are short: layer norm, dropout, the served 8-bit product.  Argument checks,
+// Tensor side of the head operators: layer norm, dropout, the 8-bit product served and trained.  Argument checks,
 // output allocation and the autograd nodes run here instead of in Python, whose interpreter time was several times the
 // kernels' (forward and backward of a layer norm of 64 x 4096: 121 us, 12 of them on the GPU).  The kernels are reached through
 // the addresses of the C ABI's entry points (include/yfs.h) that the Python side hands over from the library it has loaded.
@@ -31,6 +31,11 @@ struct Entries {
     decltype(&yfs_dropout_bwd) drop_bwd;
     decltype(&yfs_fp8_matmul) matmul;
     decltype(&yfs_fp8_matmul_workspace_bytes) matmul_ws;
+    decltype(&yfs_fp8_linear_saved_bytes) lin_saved;
+    decltype(&yfs_fp8_linear_fwd_workspace_bytes) lin_fwd_ws;
+    decltype(&yfs_fp8_linear_bwd_workspace_bytes) lin_bwd_ws;
+    decltype(&yfs_fp8_linear_fwd) lin_fwd;
+    decltype(&yfs_fp8_linear_bwd) lin_bwd;
 } yfs;
 
 [[noreturn]] void fail(const std::string& what) { throw YfsException(what); }
@@ -240,6 +245,95 @@ Tensor fp8_matmul(const Tensor& x, const Tensor& data, const Tensor& scale, int6
     return y;
 }
 
+// ---- 8-bit linear layer, trained -------------------------------------------------------------------------------------
+Tensor bytes_like(const Tensor& t, size_t n) { return n ? at::empty({(int64_t)n}, t.options().dtype(at::kByte)) : Tensor(); }
+void* mptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+
+// needs: YFS_NEED_* of the backward pass; saved: what it will multiply
+Tensor linear_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, int needs, Tensor& saved) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t n = weight.size(0), k = weight.size(1);
+    const Rows r(x), w(weight);
+    const Tensor b = f32_vector(bias);
+    at::DimVector sizes(x.sizes());
+    sizes.back() = n;
+    Tensor y = at::empty(sizes, x.options());
+    if (r.rows) {
+        const size_t kept = yfs.lin_saved(r.rows, n, k, needs), space = yfs.lin_fwd_ws(r.rows, n, k);
+        saved = bytes_like(x, kept);
+        const Tensor ws = bytes_like(x, space);
+        check(yfs.lin_fwd(ptr(r.t), code(x.scalar_type()), r.stride, ptr(w.t), code(weight.scalar_type()), w.stride, f32(b), mptr(y),
+                          code(x.scalar_type()), r.rows, n, k, needs, mptr(saved), kept, mptr(ws), space, stream_of(x)),
+              "yfs_fp8_linear_fwd");
+    }
+    return y;
+}
+
+struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias_, int64_t needs) {
+        const Tensor bias = get(bias_);
+        Tensor saved, y = linear_forward(x, weight, bias, (int)needs, saved);
+        ctx->save_for_backward({saved});
+        ctx->saved_data["x"] = x.sizes().vec();
+        ctx->saved_data["nk"] = std::vector<int64_t>{x.numel() / weight.size(1), weight.size(0), weight.size(1), needs, (int64_t)weight.scalar_type(),
+                                                     bias.defined() ? (int64_t)bias.scalar_type() : -1};
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("fp8_linear");
+        const Tensor saved = ctx->get_saved_variables()[0], &dy = grads[0];
+        if (!dy.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+        const auto nk = ctx->saved_data["nk"].toIntVector();
+        const int64_t m = nk[0], n = nk[1], k = nk[2];
+        const int needs = (int)nk[3];
+        const bool need_b = nk[5] >= 0 && ctx->needs_input_grad(2);
+        const c10::DeviceGuard guard(dy.device());
+        const auto f = dy.options().dtype(at::kFloat);
+        Tensor dx, dw, db;
+        if (needs & YFS_NEED_DX) dx = at::empty(ctx->saved_data["x"].toIntVector(), dy.options());
+        if (needs & YFS_NEED_DW) dw = m ? at::empty({n, k}, f) : at::zeros({n, k}, f);
+        if (m == 0) {
+            if (need_b) db = at::zeros({n}, f);
+        } else if (!needs) {
+            if (need_b) db = dy.reshape({m, n}).to(at::kFloat).sum(0);
+        } else {
+            const Rows d(dy);
+            if (needs & YFS_NEED_DB) db = at::empty({n}, f);
+            const size_t space = yfs.lin_bwd_ws(m, n, k, needs);
+            const Tensor ws = bytes_like(dy, space);
+            check(yfs.lin_bwd(ptr(d.t), code(dy.scalar_type()), d.stride, mptr(dx), code(dy.scalar_type()), f32(dw), 0, f32(db), 0, m, n, k,
+                              needs, ptr(saved), (size_t)saved.numel(), mptr(ws), space, stream_of(dy)),
+                  "yfs_fp8_linear_bwd");
+        }
+        if (dw.defined() && nk[4] != (int64_t)at::kFloat) dw = dw.to((at::ScalarType)nk[4]);
+        if (db.defined() && nk[5] != (int64_t)at::kFloat) db = db.to((at::ScalarType)nk[5]);
+        return {dx, dw, db, Tensor()};
+    }
+};
+
+void fp8_linear_check(const Tensor& x, const Tensor& weight, const OptTensor& bias_) {
+    if (weight.dim() != 2 || weight.size(0) == 0 || weight.size(1) == 0 || code(weight.scalar_type()) < 0)
+        fail(c10::str("fp8_linear: expected a non-empty fp32, bf16 or fp16 weight matrix, got ", str(weight)));
+    if (x.dim() == 0 || x.size(-1) != weight.size(1) || code(x.scalar_type()) < 0)
+        fail(c10::str("fp8_linear: x fp32, bf16 or fp16 [..., ", weight.size(1), "] expected, got ", str(x)));
+    const Tensor b = get(bias_);
+    if (b.defined() && (b.dim() != 1 || b.size(0) != weight.size(0) || !b.is_floating_point()))
+        fail(c10::str("fp8_linear: bias must be floating point [", weight.size(0), "], got ", str(b)));
+    on_one_gpu("fp8_linear", {&x, &weight, &b});
+}
+Tensor fp8_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
+    fp8_linear_check(x, weight, bias);
+    const Tensor b = get(bias);
+    const bool grad = at::GradMode::is_enabled(), gx = grad && x.requires_grad(), gw = grad && weight.requires_grad(),
+               gb = grad && b.defined() && b.requires_grad();
+    // db alone is a sum of dy: nothing is kept for it
+    const int needs = (gx ? YFS_NEED_DX : 0) | (gw ? YFS_NEED_DW : 0) | (gb && (gx || gw) ? YFS_NEED_DB : 0);
+    if (gx || gw || gb) return Fp8LinearFn::apply(x, weight, bias, (int64_t)needs);
+    at::AutoDispatchBelowADInplaceOrView below;
+    Tensor saved;
+    return linear_forward(x, weight, b, 0, saved);
+}
+
 template <typename F>
 void take(F& f, const py::dict& at, const char* name) { f = reinterpret_cast<F>(at[name].cast<uintptr_t>()); }
 
@@ -253,6 +347,11 @@ void init(const py::dict& addresses, const py::object& error) {
     take(yfs.drop_bwd, addresses, "yfs_dropout_bwd");
     take(yfs.matmul, addresses, "yfs_fp8_matmul");
     take(yfs.matmul_ws, addresses, "yfs_fp8_matmul_workspace_bytes");
+    take(yfs.lin_saved, addresses, "yfs_fp8_linear_saved_bytes");
+    take(yfs.lin_fwd_ws, addresses, "yfs_fp8_linear_fwd_workspace_bytes");
+    take(yfs.lin_bwd_ws, addresses, "yfs_fp8_linear_bwd_workspace_bytes");
+    take(yfs.lin_fwd, addresses, "yfs_fp8_linear_fwd");
+    take(yfs.lin_bwd, addresses, "yfs_fp8_linear_bwd");
     g_error = error.inc_ref().ptr();   // for the life of the process
 }
 }  // namespace
@@ -269,4 +368,6 @@ PYBIND11_MODULE(_binding, m) {
     m.def("layer_norm", &layer_norm);
     m.def("dropout", &dropout);
     m.def("fp8_matmul", &fp8_matmul);
+    m.def("fp8_linear", &fp8_linear);
+    m.def("fp8_linear_check", &fp8_linear_check);
 }

@@ -122,7 +122,10 @@ def fp8_matmul(x, w, bias=None, slope=None, out_dtype=None):
     return (L._binding or L.binding()).fp8_matmul(x, w.data, w.scale, w.k, bias, slope, out_dtype)
 
 
-class _Fp8LinearFn(torch.autograd.Function):
+class _SinkLinearFn(torch.autograd.Function):
+    """The node of a layer whose gradients go straight into their place in an optimiser's arena (train.FlatSGD); any other
+    weight's is the extension module's."""
+
     @staticmethod
     def forward(ctx, x, weight, bias):
         n, k = weight.shape
@@ -200,12 +203,11 @@ def fp8_linear(x, weight, bias=None):
     """y [..., n] = Q(x) Q(weight)^T + bias, differentiable, in x's dtype: x [..., k] and weight [n, k] fp32, bf16 or fp16.
     The backward pass multiplies in 8 bits too: dx = Q(dy) Q(weight), dW = Q(dy^T) Q(x^T)^T (summed in fp32, as the bias's
     gradient is); for it the transposed 8-bit weight and x are kept, not the 16-bit x."""
-    _check_weight(weight)
-    if x.dim() == 0 or x.shape[-1] != weight.shape[1] or x.dtype not in L.DTYPES:
-        raise L.YfsError(f"fp8_linear: x fp32, bf16 or fp16 [..., {weight.shape[1]}] expected, got {x.dtype} {tuple(x.shape)}")
-    _bias(bias, weight.shape[0], "fp8_linear")
-    L.require_cuda(x, weight, bias)
-    return _Fp8LinearFn.apply(x, weight, bias)
+    ext = L._binding or L.binding()
+    if getattr(weight, "_yfs_grad_sink", None) is None and getattr(bias, "_yfs_grad_sink", None) is None:
+        return ext.fp8_linear(x, weight, bias)
+    ext.fp8_linear_check(x, weight, bias)
+    return _SinkLinearFn.apply(x, weight, bias)
 
 
 class Fp8Linear(nn.Linear):
