@@ -345,7 +345,9 @@ int yfs_mask_to_boxes_u8(const uint8_t *mask, int64_t N, int H, int W, int CH, c
 int yfs_anchor_assign_f32(const float *wh, int64_t n, const float *anchors, int k, int32_t *assign, float *best_iou,
                           void *stream);
 
-/* ---- operators of the fully connected head (no reference code; the head is yolo_toy_regressor_torch.py:258-266) --------- */
+/* ---- operators of the fully connected head (no reference code; the head is yolo_toy_regressor_torch.py:258-266) ---------
+ * Outputs and workspaces overlap neither the inputs nor each other, where nothing else is said.  Calls that run at one time
+ * need workspaces of their own; no call keeps anything. */
 
 typedef enum { YFS_F32 = 0, YFS_BF16 = 1, YFS_F16 = 2 } yfs_dtype;
 
@@ -397,7 +399,7 @@ int yfs_fp8_matmul(const void *x, int x_dtype, int64_t ld, const void *wq, const
 /* Layer norm over the last axis: y = (x - mu) / sqrt(v + eps) * w + b with the row's mean mu and biased variance v, all in
  * fp32 with one rounding at the end.  x [rows, cols] with x_stride elements from row to row (0: one row for all), y [rows,
  * cols] dense, both `dtype`; w, b [cols] fp32 or NULL (ones / zeros); mean, rstd [rows] fp32 or NULL: what the backward
- * pass needs. */
+ * pass needs.  cols < 2^28. */
 int yfs_layer_norm_fwd(const void *x, int64_t x_stride, const float *w, const float *b, void *y, float *mean, float *rstd,
                        int64_t rows, int64_t cols, float eps, int dtype, void *stream);
 /* g = dy w; dx = rstd (g - mean(g) - h mean(g h)) with h = (x - mean) rstd; dw = sum over rows of dy h; db = sum over rows

@@ -373,3 +373,29 @@ def test_second_derivative_is_refused():
         with pytest.raises(RuntimeError):
             g, = torch.autograd.grad(f().sum(), x, create_graph=True)
             g.sum().backward()
+
+
+def test_width_limit():
+    import yolo_from_scratch_amd as y
+    lib, p, n = y.lib(), 4096, 1 << 28
+    assert lib.yfs_layer_norm_fwd(p, n, None, None, p, None, None, 1, n, 1e-5, 0, None) == -1
+    assert lib.yfs_layer_norm_bwd(p, n, p, n, None, p, p, p, p, p, 1, n, 0, p, 1 << 40, None) == -1
+    assert lib.yfs_layer_norm_bwd_workspace_bytes(1, n, 0) == 0
+
+
+@pytest.mark.gpu
+def test_longest_row():
+    """x = +1, -1, ...: mean 2^-28, variance 1; dy = +1, +1, -1, -1, ... has no part along 1 or h.  The sums are exact up to 2^24
+    and off by 20 steps of 2^-24 at most behind it, so that y = x and dx = dy after the rounding to bf16."""
+    import yolo_from_scratch_amd as yfs
+    n = (1 << 28) - 5
+    c = torch.arange(n, device=DEV, dtype=torch.int32)
+    x = (1 - 2 * (c % 2)).bfloat16()[None].requires_grad_()
+    dy = (1 - 2 * (c % 4 // 2)).bfloat16()[None]
+    del c
+    w, b = torch.ones(n, device=DEV, requires_grad=True), torch.zeros(n, device=DEV, requires_grad=True)
+    y = yfs.layer_norm(x, w, b, eps=0.0)
+    assert torch.equal(y, x)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert torch.equal(dx, dy) and torch.equal(db, dy[0].float())
+    assert float((dw - dy[0].float() * x[0].detach().float()).abs().max()) <= 32 * 2.0 ** -24

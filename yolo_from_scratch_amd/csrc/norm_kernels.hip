@@ -489,13 +489,14 @@ int bwd(BwdArgs g, float* part, hipStream_t s) {
 }
 
 bool known(int dtype) { return dtype == YFS_F32 || dtype == YFS_BF16 || dtype == YFS_F16; }
+constexpr long long kMostCols = 1LL << 28;   // (a launch has fewer than 2^32 threads: 8 or 4 per column of the longest rows' sums)
 }  // namespace
 
 YFS_API int yfs_layer_norm_fwd(const void* x, int64_t x_stride, const float* w, const float* b, void* y, float* mean, float* rstd,
                                int64_t rows, int64_t cols, float eps, int dtype, void* stream) {
     YFS_REQUIRE(x && y, YFS_ERR_INVALID_ARG, "yfs_layer_norm_fwd: null pointer");
-    YFS_REQUIRE(rows > 0 && cols > 0 && cols < (1LL << 30) && x_stride >= 0, YFS_ERR_INVALID_ARG,
-                "yfs_layer_norm_fwd: need rows > 0, 0 < cols < 2^30 and a row stride >= 0 (got rows=%lld cols=%lld stride=%lld)",
+    YFS_REQUIRE(rows > 0 && cols > 0 && cols < kMostCols && x_stride >= 0, YFS_ERR_INVALID_ARG,
+                "yfs_layer_norm_fwd: need rows > 0, 0 < cols < 2^28 and a row stride >= 0 (got rows=%lld cols=%lld stride=%lld)",
                 (long long)rows, (long long)cols, (long long)x_stride);
     YFS_REQUIRE(eps >= 0.0f, YFS_ERR_INVALID_ARG, "yfs_layer_norm_fwd: eps %g is negative", eps);
     YFS_REQUIRE(known(dtype), YFS_ERR_UNSUPPORTED, "yfs_layer_norm_fwd: unknown dtype %d", dtype);
@@ -507,7 +508,7 @@ YFS_API int yfs_layer_norm_fwd(const void* x, int64_t x_stride, const float* w, 
 
 // (with or without dx: the larger of the two)
 YFS_API size_t yfs_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols, int dtype) {
-    if (rows <= 0 || cols <= 0 || cols >= (1LL << 30) || !known(dtype)) return 0;
+    if (rows <= 0 || cols <= 0 || cols >= kMostCols || !known(dtype)) return 0;
     size_t most = 0;
     for (int dx = 0; dx < 2; ++dx) {
         const BwdPlan p = bwd_plan(rows, (int)cols, dtype == YFS_F32 ? 4 : 2, dx);
@@ -521,8 +522,8 @@ YFS_API int yfs_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x,
                                const float* rstd, void* dx, float* dw, float* db, int64_t rows, int64_t cols, int dtype,
                                void* workspace, size_t workspace_bytes, void* stream) {
     YFS_REQUIRE(dy && x && mean && rstd, YFS_ERR_INVALID_ARG, "yfs_layer_norm_bwd: null pointer");
-    YFS_REQUIRE(rows > 0 && cols > 0 && cols < (1LL << 30) && x_stride >= 0 && dy_stride >= 0, YFS_ERR_INVALID_ARG,
-                "yfs_layer_norm_bwd: need rows > 0, 0 < cols < 2^30 and row strides >= 0 (got rows=%lld cols=%lld)", (long long)rows,
+    YFS_REQUIRE(rows > 0 && cols > 0 && cols < kMostCols && x_stride >= 0 && dy_stride >= 0, YFS_ERR_INVALID_ARG,
+                "yfs_layer_norm_bwd: need rows > 0, 0 < cols < 2^28 and row strides >= 0 (got rows=%lld cols=%lld)", (long long)rows,
                 (long long)cols);
     YFS_REQUIRE(known(dtype), YFS_ERR_UNSUPPORTED, "yfs_layer_norm_bwd: unknown dtype %d", dtype);
     const size_t need = (dw || db) ? yfs_layer_norm_bwd_workspace_bytes(rows, cols, dtype) : 0;
