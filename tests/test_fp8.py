@@ -482,3 +482,57 @@ def test_frozen_layers():
     state = {k: v.clone() for k, v in net.state_dict().items()}
     net.load_state_dict(state)
     assert torch.equal(net(x), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k", [(5, 300), (20, 300), (300, 200)])
+def test_smallest_scales(m, k):
+    """Blocks around the smallest scale, 2^-127, and below it.  A widened operand is off by half the smallest bf16, 2^-134, at most."""
+    import yolo_from_scratch_amd as yfs
+    x = _matrix(m, k, 21, device="cpu")
+    for i, e in enumerate((-118, -122, -126, -130, -136)):
+        x[i::5] *= 2.0 ** e / x[i::5].abs().amax(1, keepdim=True)
+    x[:, 128:] *= 2.0 ** -3
+    x = x.to(DEV)
+    w = _matrix(70, k, 22) * 2.0 ** 100
+    wq = yfs.quantize_fp8(w)
+    xn, wn = hr.rounded(_np(x), 1, 128), hr.rounded(_np(w), 128, 128)
+    ref = xn @ wn.T
+    for out in (torch.float32, torch.bfloat16):
+        tol = _tolerance(xn, wn, ref, out)
+        if out == torch.float32:
+            tol = tol + 2.0 ** -134 * np.abs(wn).sum(1)
+        _close(_np(yfs.fp8_matmul(x, wq, out_dtype=out)), ref, tol, str(out))
+
+
+@pytest.mark.gpu
+def test_serving_a_layer_that_trains_keeps_nothing():
+    """A layer bound to an optimiser's arena, called without gradients, does what fp8_linear of plain tensors does."""
+    import yolo_from_scratch_amd as yfs
+    from yolo_from_scratch_amd.train import FlatSGD
+    lin = yfs.Fp8Linear(300, 70).to(DEV)
+    x = _matrix(33, 300, 23, torch.bfloat16)
+    FlatSGD(lin.parameters(), lr=0.1)
+    with torch.no_grad():
+        y = lin(x)
+        assert y.grad_fn is None and torch.equal(y, yfs.fp8_linear(x, lin.weight.clone(), lin.bias.clone()))
+    assert torch.equal(lin(x), y)
+
+
+def test_freeze_refuses_a_layer_alone():
+    import yolo_from_scratch_amd as yfs
+    with pytest.raises(yfs.YfsError, match="FrozenFp8Linear"):
+        yfs.freeze_fp8(torch.nn.Linear(4, 4))
+
+
+@pytest.mark.gpu
+def test_freeze_converts_a_shared_layer_once_and_all_or_none():
+    import yolo_from_scratch_amd as yfs
+    lin = torch.nn.Linear(64, 64).to(DEV)
+    net = torch.nn.Sequential(lin, torch.nn.ReLU(), lin, torch.nn.Sequential(lin))
+    yfs.freeze_fp8(net)
+    assert isinstance(net[0], yfs.FrozenFp8Linear) and net[2] is net[0] and net[3][0] is net[0]
+    net = torch.nn.Sequential(torch.nn.Linear(8, 8).to(DEV), torch.nn.Linear(8, 8).double().to(DEV))
+    with pytest.raises(yfs.YfsError):
+        yfs.freeze_fp8(net)
+    assert isinstance(net[0], torch.nn.Linear) and net.training

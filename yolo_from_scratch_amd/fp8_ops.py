@@ -204,7 +204,7 @@ def fp8_linear(x, weight, bias=None):
     The backward pass multiplies in 8 bits too: dx = Q(dy) Q(weight), dW = Q(dy^T) Q(x^T)^T (summed in fp32, as the bias's
     gradient is); for it the transposed 8-bit weight and x are kept, not the 16-bit x."""
     ext = L._binding or L.binding()
-    if getattr(weight, "_yfs_grad_sink", None) is None and getattr(bias, "_yfs_grad_sink", None) is None:
+    if (getattr(weight, "_yfs_grad_sink", None) is None and getattr(bias, "_yfs_grad_sink", None) is None) or not torch.is_grad_enabled():
         return ext.fp8_linear(x, weight, bias)
     ext.fp8_linear_check(x, weight, bias)
     return _SinkLinearFn.apply(x, weight, bias)
@@ -247,12 +247,18 @@ class FrozenFp8Linear(nn.Module):
 
 def freeze_fp8(model):
     """Replaces every linear layer of ``model`` (on the GPU) by its 8-bit form for serving, a fused LeakyReLU included, and
-    puts the model into eval mode.  In place; returns the model."""
+    puts the model into eval mode.  In place, all layers or (where one cannot be converted) none; a layer that stands in several
+    places is converted once.  Returns the model."""
     from .model import HipLinear
     from .train import bf16_shadow
-    for module in list(model.modules()):
-        for name, child in list(module.named_children()):
-            if isinstance(child, nn.Linear):
-                bf16_shadow(child.weight)          # a step that is still running on the weight is waited for
-                module._modules[name] = FrozenFp8Linear(child, child.fused_act if isinstance(child, HipLinear) else None)
+    if isinstance(model, nn.Linear):
+        raise L.YfsError("freeze_fp8: replaces the linear layers inside a module; for a layer alone: FrozenFp8Linear(layer)")
+    places = [(m, name, c) for m in model.modules() for name, c in m._modules.items() if isinstance(c, nn.Linear)]
+    frozen = {}
+    for _, _, child in places:
+        if child not in frozen:
+            bf16_shadow(child.weight)          # a step that is still running on the weight is waited for
+            frozen[child] = FrozenFp8Linear(child, child.fused_act if isinstance(child, HipLinear) else None)
+    for module, name, child in places:
+        module._modules[name] = frozen[child]
     return model.eval()
