@@ -198,3 +198,12 @@ def test_module():
     assert torch.equal(m(x), torch.nn.functional.leaky_relu(x, 0.1))
     plain = yfs.HipDropout(0.5).eval()
     assert plain(x) is x
+
+
+@pytest.mark.gpu
+def test_any_whole_number_is_a_seed():
+    import yolo_from_scratch_amd as yfs
+    x = torch.ones(1000, device=DEV)
+    want = yfs.dropout(x, 0.5, 7)
+    assert torch.equal(yfs.dropout(x, 0.5, np.int64(7)), want) and torch.equal(yfs.dropout(x, 0.5, 7 + (1 << 64)), want)
+    assert torch.equal(yfs.dropout(x, 0.5, -1), yfs.dropout(x, 0.5, (1 << 64) - 1))

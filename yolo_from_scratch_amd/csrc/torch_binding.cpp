@@ -206,8 +206,10 @@ Tensor dropout(const Tensor& x, double p, const py::object& seed, double slope) 
     if (THPVariable_Check(seed.ptr())) {
         dev = THPVariable_Unpack(seed.ptr());
         if (dev.scalar_type() != at::kLong || dev.numel() != 1) fail(c10::str("dropout: a seed tensor must hold one int64, got ", str(dev)));
-    } else if (PyLong_Check(seed.ptr())) {
-        value = (int64_t)PyLong_AsUnsignedLongLongMask(seed.ptr());
+    } else if (PyIndex_Check(seed.ptr())) {
+        const py::object whole = py::reinterpret_steal<py::object>(PyNumber_Index(seed.ptr()));
+        if (!whole) throw py::error_already_set();
+        value = (int64_t)PyLong_AsUnsignedLongLongMask(whole.ptr());
     } else fail(c10::str("dropout: seed must be an int or an int64 tensor, got ", Py_TYPE(seed.ptr())->tp_name));
     on_one_gpu("dropout", {&x, &dev});
     if (at::GradMode::is_enabled() && x.requires_grad()) return DropoutFn::apply(x, p, slope, value, dev.defined() ? OptTensor(dev) : std::nullopt);
