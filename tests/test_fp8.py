@@ -536,3 +536,64 @@ def test_freeze_converts_a_shared_layer_once_and_all_or_none():
     with pytest.raises(yfs.YfsError):
         yfs.freeze_fp8(net)
     assert isinstance(net[0], torch.nn.Linear) and net.training
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(64, 300, 1000), (65, 300, 1000), (1, 4096, 4096), (33, 1, 50176), (64, 40, 50176), (17, 1470, 130)])
+def test_linear_around_the_rows_that_are_quantised_in_the_product(m, n, k):
+    """Up to 64 rows the weights are quantised by the workgroups that multiply them: the forward pass is that of stored weights,
+    to the rounding of the output, with and without gradients, and the transposed operands are those of the other form."""
+    import yolo_from_scratch_amd as yfs
+    x, w, b = _matrix(m, k, 31, torch.bfloat16), _matrix(n, k, 32), torch.randn(n, device=DEV)
+    dy = _matrix(m, n, 33, torch.bfloat16)
+    xn, wn, dn = hr.rounded(_np(x), 1, 128), hr.rounded(_np(w), 128, 128), hr.rounded(_np(dy), 1, 128)
+    ref = xn @ wn.T + _np(b)
+    for wt in (w, w.bfloat16(), w.half()):
+        wr = wn if wt is w else hr.rounded(_np(wt), 128, 128)
+        r = ref if wt is w else xn @ wr.T + _np(b)
+        y = yfs.fp8_linear(x, wt, b)
+        _close(_np(y), r, _tolerance(xn, wr, r, torch.bfloat16, _np(b)), f"y, {wt.dtype} weights")
+    y32 = yfs.fp8_linear(x.float(), w, b)
+    _close(_np(y32), ref, _tolerance(xn, wn, ref, torch.float32, _np(b)), "fp32 y")
+    x, w = x.requires_grad_(), w.requires_grad_()
+    y = yfs.fp8_linear(x, w, b)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    _close(_np(y), ref, _tolerance(xn, wn, ref, torch.bfloat16, _np(b)), "y")
+    plain = dn @ wn
+    _close(_np(dx), plain, _tolerance(dn, wn.T, plain, torch.bfloat16), "dx")
+    dt, xt = hr.rounded(_np(dy).T, 1, 128), hr.rounded(_np(x).T, 1, 128)
+    plain = dt @ xt.T
+    _close(_np(dw), plain, _tolerance(dt, xt, plain, torch.float32), "dw")
+    only = torch.autograd.grad(yfs.fp8_linear(x, w.detach(), b), x, dy)[0]
+    assert torch.equal(only, dx)
+    only = torch.autograd.grad(yfs.fp8_linear(x.detach(), w, b), w, dy)[0]
+    assert torch.equal(only, dw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [30011, 30016])
+def test_large_weights_that_pass_the_caches_by(k):
+    """From 128 MiB on weights are read and their gradients written past the caches where rows begin on a line of 128 bytes: the
+    same values as in parts below that size."""
+    import yolo_from_scratch_amd as yfs
+    n = 1160                              # 139 MB
+    w = _matrix(n, k, 41).requires_grad_()
+    for m in (40, 200):
+        x, dy = _matrix(m, k, 42, torch.bfloat16), _matrix(m, n, 43, torch.bfloat16)
+        y = yfs.fp8_linear(x, w)
+        dw, = torch.autograd.grad(y, w, dy)
+        for lo, hi in ((0, 640), (640, 1160)):
+            part = w.detach()[lo:hi].contiguous().requires_grad_()
+            yp = yfs.fp8_linear(x, part)
+            dp, = torch.autograd.grad(yp, part, dy[:, lo:hi].contiguous())
+            # the reduction is split by the count of columns, so y may be rounded the other way
+            assert torch.equal(dp, dw[lo:hi]) and float((yp.float() - y[:, lo:hi].float()).detach().abs().max()) <= 2.0 ** -7 * float(y.detach().abs().max())
+    from yolo_from_scratch_amd.train import FlatSGD
+    lin = yfs.Fp8Linear(k, n, bias=False).to(DEV)
+    with torch.no_grad():
+        lin.weight.copy_(w)
+    FlatSGD(lin.parameters(), lr=0.1)
+    lin(x).backward(dy)
+    assert torch.equal(lin.weight.grad, dw)
+    lin(x).backward(dy)
+    assert torch.equal(lin.weight.grad, dw + dw)

@@ -36,6 +36,14 @@ __device__ __forceinline__ int scale_exponent(float amax) {
     return u == 0 ? 0 : (e < -127 ? -127 : e);
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }   // -126 <= e <= 127
+
+// Weights that are quantised and weight gradients go past the caches from half of the 256 MB on that the last of them holds.  Weights of
+// 822 MB read through it push out their 8-bit form, which the backward pass reads next (64 x 50176 x 4096: dx 57 us, 33 with the
+// weights read past it), and as many bytes of gradients left in it are written back while the next kernels run (the quantiser behind
+// them 251 us, 217).  Only where rows begin on a line: elsewhere parts of lines are fetched or written twice (a training step at
+// 184 x 4965 x 35251: 718 us, 697 through the caches; its quantiser at 184 x 4992 x 35200 the other way round, 192 against 235).
+__host__ __device__ inline bool past_caches(long long row_bytes, long long bytes) { return bytes >= (128LL << 20) && row_bytes % 128 == 0; }
+
 __device__ __forceinline__ float finite_abs(float v) {
     const float a = fabsf(v);
     return a < __builtin_inff() ? a : 0.0f;
@@ -54,7 +62,21 @@ struct QuantArgs {
     float* colsum;             // [ceil(M/128), K] sums of x over 128 rows each, or NULL
     int groups, groups_t;      // 64-row groups of the packed planes of q and qt
     int row_blocks;            // workgroups that quantise by rows
+    bool once;                 // weights: read past the caches
 };
+
+// 8 x 8 weights of a thread: rows m .. and columns k .. of [M, K], zeros outside
+template <typename T>
+__device__ __forceinline__ void load_block(const QuantArgs& g, long long m, long long k, float (&v)[8][8]) {
+    const T* p = (const T*)g.x + m * g.ld + k;
+    if (g.once) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) load_vec8_once(p + i * g.ld, m + i < g.M ? g.K - k : 0, v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) load_vec8(p + i * g.ld, m + i < g.M ? g.K - k : 0, v[i]);
+    }
+}
 
 // Weights: one workgroup and one scale per 128 x 128 tile, 8 x 8 elements per thread; the transpose leaves through LDS.
 template <typename T, bool COLQ>
@@ -70,8 +92,7 @@ __global__ void __launch_bounds__(256) quant_block_kernel(QuantArgs g) {
     const long long k0 = kb * 128 + cg * 8, m0 = mb * 128 + rg * 8;
     const long long ldq = pad128(g.K), ldt = pad128(g.M);
     float v[8][8], a = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) load_vec8((const T*)g.x + (m0 + i) * g.ld + k0, m0 + i < g.M ? g.K - k0 : 0, v[i]);
+    load_block<T>(g, m0, k0, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -302,6 +323,7 @@ __device__ __forceinline__ void store4(const GemmArgs& g, long long m, long long
 template <int BM, int BN, int NT>
 __device__ __forceinline__ void store_tile(const GemmArgs& g, const unsigned char* smem, long long m0, long long n0) {
     constexpr int PER = BN / 4, PITCH = BN * 4 + 16;
+    const bool once = past_caches(g.N * 4, g.M * g.N * 4);
 #pragma unroll 4
     for (int id = threadIdx.x; id < BM * PER; id += NT) {
         const int r = id / PER, ch = id % PER;
@@ -310,7 +332,8 @@ __device__ __forceinline__ void store_tile(const GemmArgs& g, const unsigned cha
         f32x4 t = *reinterpret_cast<const f32x4*>(smem + r * PITCH + ch * 16);
         float* o = (float*)g.out + m * g.N + n;
         if (g.accumulate) t += load4((const float*)g.out + m * g.N, n, g.N);
-        if (n + 4 <= g.N) __builtin_memcpy(o, &t, 16);
+        if (n + 4 <= g.N && once) __builtin_nontemporal_store(__builtin_bit_cast(i32x4, t), (yfs_int4_any*)o);
+        else if (n + 4 <= g.N) __builtin_memcpy(o, &t, 16);
         else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -749,6 +772,121 @@ __global__ void __launch_bounds__(1024) fp8_rows_kernel(GemmArgs g, const T* x, 
     }
 }
 
+// A training step's forward pass for at most 64 rows: bound by the bytes of the weights in their own type, so they are
+// quantised, transposed for the backward pass and multiplied while they are on the chip.  A workgroup takes 128 columns of y and
+// per_split blocks of the reduction; per block the 128 x 128 weights are read once, leave through LDS as 8-bit columns (qt, for dx),
+// and from LDS as rows into the products: a wave owns 32 columns of all 64 rows.  The partial sums are joined by fp8_join_kernel.
+template <typename T, typename TO>
+__global__ void __launch_bounds__(256) fp8_train_rows_kernel(GemmArgs g, QuantArgs w) {
+    constexpr bool EXACT = sizeof(TO) == 4;
+    __shared__ float red[4];
+    __shared__ __attribute__((aligned(16))) unsigned char wt[128 * 128], xt[64 * 128], tt[128 * 144];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, frow = lane & 15, fk = lane >> 4;
+    const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4;
+    const int down = (int)((g.N + 127) >> 7), nb = (int)blockIdx.x % down, split = (int)blockIdx.x / down;
+    const int kb0 = split * g.per_split, kb1 = kb0 + g.per_split < g.kblocks ? kb0 + g.per_split : g.kblocks;
+    const long long n0 = nb * 128LL, m0 = n0 + rg * 8, ldt = pad128(g.N), ldx = g.kblocks * 128LL;
+    auto fragment = [&](const unsigned char* base, int row) {
+        const i32x4 lo = *reinterpret_cast<const i32x4*>(base + row * 128 + ((fk ^ (row & 7)) * 16));
+        const i32x4 hi = *reinterpret_cast<const i32x4*>(base + row * 128 + (((4 + fk) ^ (row & 7)) * 16));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    f32x4 acc[2][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) (&acc[0][0])[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int kb = kb0; kb < kb1; ++kb) {
+        const long long k0 = kb * 128LL + cg * 8;
+        float v[8][8], a = 0.0f;
+        load_block<T>(w, m0, k0, v);
+        i32x4 xv[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {   // 64 rows of x, 16 bytes a thread and half
+            const int row = i * 32 + (threadIdx.x >> 3);
+            xv[i] = (i32x4){0, 0, 0, 0};
+            if (row < g.M) xv[i] = *reinterpret_cast<const i32x4*>(g.a + row * ldx + kb * 128LL + (threadIdx.x & 7) * 16);
+        }
+        const int sa = *reinterpret_cast<const int*>(g.as + (long long)kb * g.groups_a * 64 + frow * 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(v[i][j]));
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+        if (lane == 0) red[wave] = a;
+        __syncthreads();   // (and every wave has left the block before this one)
+        const int e = scale_exponent(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+        const float f = pow2(-e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = rg * 8 + i;
+            *reinterpret_cast<uint2*>(wt + row * 128 + (((cg >> 1) ^ (row & 7)) * 16) + (cg & 1) * 8) =
+                make_uint2(pack4(v[i][0] * f, v[i][1] * f, v[i][2] * f, v[i][3] * f), pack4(v[i][4] * f, v[i][5] * f, v[i][6] * f, v[i][7] * f));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = i * 32 + (threadIdx.x >> 3);
+            *reinterpret_cast<i32x4*>(xt + row * 128 + (((threadIdx.x & 7) ^ (row & 7)) * 16)) = xv[i];
+        }
+        if (w.qt) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<uint2*>(tt + (cg * 8 + j) * 144 + rg * 8) =
+                    make_uint2(pack4(v[0][j] * f, v[1][j] * f, v[2][j] * f, v[3][j] * f), pack4(v[4][j] * f, v[5][j] * f, v[6][j] * f, v[7][j] * f));
+        }
+        __syncthreads();
+        if (w.qt) {
+            if (threadIdx.x == 0) w.st[kb * (ldt >> 7) + nb] = (unsigned char)(e + 127);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = i * 32 + (threadIdx.x >> 3), ch = threadIdx.x & 7;
+                const long long k = kb * 128LL + c;
+                if (k < w.K)
+                    *reinterpret_cast<i32x4*>(w.qt + k * ldt + n0 + ch * 16) = *reinterpret_cast<const i32x4*>(tt + c * 144 + ch * 16);
+            }
+        }
+        i32x8 fa[4], fb[2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fa[j] = fragment(xt, j * 16 + frow);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) fb[i] = fragment(wt, wave * 32 + i * 16 + frow);
+        const int sb = e + 127;
+        if constexpr (EXACT) {
+            bf16x8 wb[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) widen(fb[i], __uint_as_float((unsigned)sb << 23), wb[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                bf16x8 wa[4];
+                widen(fa[j], __uint_as_float((((unsigned)sa >> (8 * j)) & 255u) << 23), wa);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[i][q], wa[q], acc[i][j], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                acc[i][0] = mfma_fp8<0, 0>(fb[i], fa[0], acc[i][0], sb, sa);
+                acc[i][1] = mfma_fp8<0, 1>(fb[i], fa[1], acc[i][1], sb, sa);
+                acc[i][2] = mfma_fp8<0, 2>(fb[i], fa[2], acc[i][2], sb, sa);
+                acc[i][3] = mfma_fp8<0, 3>(fb[i], fa[3], acc[i][3], sb, sa);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const long long m = j * 16 + frow;
+        if (m >= g.M) continue;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const long long n = n0 + wave * 32 + i * 16 + fk * 4;
+            if (n >= g.N) continue;
+            if (g.splits > 1) store_part(g, split, m, n, acc[i][j]);
+            else store4<TO>(g, m, n, acc[i][j]);
+        }
+    }
+}
+
 // joins the partial sums of the splits in their order
 template <typename TO>
 __global__ void __launch_bounds__(256) fp8_join_kernel(GemmArgs g) {
@@ -756,11 +894,9 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(GemmArgs g) {
     for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long long)gridDim.x * 256) {
         const long long m = id / per_row, n = (id - m * per_row) * 4;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < g.splits; ++s) {
-            const float* p = g.part + ((long long)s * g.M + m) * g.N + n;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] += n + r < g.N ? p[r] : 0.0f;
-        }
+        const float* p = g.part + m * g.N;
+#pragma unroll 8
+        for (int s = 0; s < g.splits; ++s) v += load4(p + s * g.M * g.N, n, g.N);
         store4<TO>(g, m, n, v);
     }
 }
@@ -919,6 +1055,32 @@ int matmul_rows(const GemmArgs& g, const Plan& p, const void* x, long long ldx, 
     return out_dtype == YFS_BF16 ? matmul_rows<T, bf16_t>(g, p, x, ldx, K, s) : matmul_rows<T, _Float16>(g, p, x, ldx, K, s);
 }
 
+// Rows that fp8_train_rows_kernel takes, and its plan: two workgroups per CU, two blocks or more each
+constexpr int kTrainRows = 64;
+Plan plan_train_rows(long long N, int kblocks) {
+    Plan p = {3, 64, 128, 1, kblocks, 0};
+    long long s = 2 * kCUs / yfs_cdiv(N, 128);
+    if (s > kblocks / 2) s = kblocks / 2;
+    if (s > 128) s = 128;
+    set_splits(p, s, kblocks);
+    return p;
+}
+template <typename T>
+int train_rows(GemmArgs g, const QuantArgs& w, int out_dtype, hipStream_t s) {
+    const dim3 grid((unsigned)(yfs_cdiv(g.N, 128) * g.splits));
+    if (out_dtype == YFS_F32) fp8_train_rows_kernel<T, float><<<grid, 256, 0, s>>>(g, w);
+    else if (out_dtype == YFS_BF16) fp8_train_rows_kernel<T, bf16_t><<<grid, 256, 0, s>>>(g, w);
+    else fp8_train_rows_kernel<T, _Float16><<<grid, 256, 0, s>>>(g, w);
+    YFS_CHECK_LAUNCH("fp8_train_rows_kernel");
+    yfs_note_kernel("fp8_train_rows_kernel<splits%d>", g.splits);
+    if (out_dtype == YFS_F32) return join<float>(g, s);
+    return out_dtype == YFS_BF16 ? join<bf16_t>(g, s) : join<_Float16>(g, s);
+}
+
+bool weight_once(const void* w, int dtype, long long ld, long long N, long long K) {
+    const long long size = dtype == YFS_F32 ? 4 : 2;
+    return past_caches((long long)(reinterpret_cast<uintptr_t>(w) & 127) + ld * size, N * K * size);
+}
 bool known(int d) { return d == YFS_F32 || d == YFS_BF16 || d == YFS_F16; }
 constexpr int64_t kMost = (1LL << 23) - 256;   // 65534 tiles of 128 rows; a tile's rows of pad128(K) bytes stay inside one buffer descriptor
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -939,7 +1101,7 @@ YFS_API int yfs_fp8_quantize_weight(const void* w, int dtype, int64_t ld, int64_
     YFS_REQUIRE(known(dtype), YFS_ERR_UNSUPPORTED, "yfs_fp8_quantize_weight: unknown dtype %d", dtype);
     REQUIRE_ALIGNED("yfs_fp8_quantize_weight", q);
     REQUIRE_ALIGNED("yfs_fp8_quantize_weight", qt);
-    const QuantArgs g = {w, ld, N, K, (unsigned char*)q, (unsigned char*)scale, (unsigned char*)qt, (unsigned char*)scale_t, nullptr, 0, 0, 0};
+    const QuantArgs g = {w, ld, N, K, (unsigned char*)q, (unsigned char*)scale, (unsigned char*)qt, (unsigned char*)scale_t, nullptr, 0, 0, 0, weight_once(w, dtype, ld, N, K)};
     return qt ? quantize_blocks<true>(g, dtype, (hipStream_t)stream) : quantize_blocks<false>(g, dtype, (hipStream_t)stream);
 }
 
@@ -956,7 +1118,7 @@ YFS_API int yfs_fp8_quantize_rows(const void* x, int dtype, int64_t ld, int64_t 
     REQUIRE_ALIGNED("yfs_fp8_quantize_rows", q);
     REQUIRE_ALIGNED("yfs_fp8_quantize_rows", qt);
     const QuantArgs g = {x, ld, M, K, (unsigned char*)q, (unsigned char*)scale, (unsigned char*)qt, (unsigned char*)scale_t, colsum,
-                         groups64(M), groups64(K), 0};
+                         groups64(M), groups64(K), 0, false};
     return quantize_rows(g, dtype, (hipStream_t)stream);
 }
 
@@ -1070,15 +1232,18 @@ struct Saved {
     }
 };
 struct ForwardSpace {
-    unsigned char *wq, *ws, *xq, *xs, *part;
+    unsigned char *wq = nullptr, *ws = nullptr, *xq, *xs, *part;
     size_t part_bytes, bytes;
     ForwardSpace(void* buf, long long M, long long N, long long K) {
         Pieces p{(unsigned char*)buf};
-        wq = p.take((size_t)(N * pad128(K)));
-        ws = p.take((size_t)(yfs_cdiv(N, 128) * yfs_cdiv(K, 128)));
+        const int kb = (int)yfs_cdiv(K, 128);
+        if (M > kTrainRows) {
+            wq = p.take((size_t)(N * pad128(K)));
+            ws = p.take((size_t)(yfs_cdiv(N, 128) * kb));
+        }
         xq = p.take((size_t)(M * pad128(K)));
-        xs = p.take((size_t)packed_bytes(M, yfs_cdiv(K, 128)));
-        part_bytes = yfs_fp8_gemm_workspace_bytes(M, N, K);
+        xs = p.take((size_t)packed_bytes(M, kb));
+        part_bytes = M > kTrainRows ? yfs_fp8_gemm_workspace_bytes(M, N, K) : ::part_bytes(plan_train_rows(N, kb), M, N);
         part = p.take(part_bytes);
         bytes = p.used;
     }
@@ -1130,6 +1295,19 @@ YFS_API int yfs_fp8_linear_fwd(const void* x, int x_dtype, int64_t ldx, const vo
                 "yfs_fp8_linear_fwd: workspace needs %zu bytes, 256-byte aligned", f.bytes);
     YFS_REQUIRE(k.bytes == 0 || (saved && saved_bytes >= k.bytes && aligned256(saved)), YFS_ERR_WORKSPACE,
                 "yfs_fp8_linear_fwd: saved needs %zu bytes, 256-byte aligned", k.bytes);
+    YFS_REQUIRE(known(w_dtype) && known(y_dtype) && ldw >= 0, YFS_ERR_UNSUPPORTED, "yfs_fp8_linear_fwd: unknown dtype %d or %d, or a negative row stride",
+                w_dtype, y_dtype);
+    if (M <= kTrainRows) {
+        const int rc = yfs_fp8_quantize_rows(x, x_dtype, ldx, M, K, f.xq, f.xs, k.xqt, k.xst, nullptr, stream);
+        if (rc != YFS_OK) return rc;
+        const Plan p = plan_train_rows(N, (int)yfs_cdiv(K, 128));
+        const GemmArgs g = {f.xq, f.xs, nullptr, nullptr, bias, y, (float*)f.part, M, N, (int)yfs_cdiv(K, 128), p.splits, p.per_split,
+                            groups64(M), 0, 0, 1.0f, 0};
+        const QuantArgs q = {w, ldw, N, K, nullptr, nullptr, k.wqt, k.wst, nullptr, 0, 0, 0, weight_once(w, w_dtype, ldw, N, K)};
+        hipStream_t s = (hipStream_t)stream;
+        if (w_dtype == YFS_F32) return train_rows<float>(g, q, y_dtype, s);
+        return w_dtype == YFS_BF16 ? train_rows<bf16_t>(g, q, y_dtype, s) : train_rows<_Float16>(g, q, y_dtype, s);
+    }
     int rc = yfs_fp8_quantize_weight(w, w_dtype, ldw, N, K, f.wq, f.ws, k.wqt, k.wst, stream);
     if (rc == YFS_OK) rc = yfs_fp8_quantize_rows(x, x_dtype, ldx, M, K, f.xq, f.xs, k.xqt, k.xst, nullptr, stream);
     if (rc == YFS_OK)

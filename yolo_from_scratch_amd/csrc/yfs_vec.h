@@ -83,3 +83,20 @@ __device__ __forceinline__ void load_vec8(const T* p, long long n, float (&v)[8]
         for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.0f;
     }
 }
+
+// The same past the caches: for an operand that is read once and would push out of them what the next kernels read
+typedef __attribute__((ext_vector_type(4), aligned(1), may_alias)) int yfs_int4_any;
+template <typename T>
+__device__ __forceinline__ void load_vec8_once(const T* p, long long n, float (&v)[8]) {
+    if (n < 8) {
+        load_vec8(p, n, v);
+        return;
+    }
+    T t[8];
+    yfs_int4_any raw[sizeof(T) / 2];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __builtin_nontemporal_load((const yfs_int4_any*)p + i);
+    __builtin_memcpy(t, raw, sizeof(t));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)t[j];
+}
