@@ -597,3 +597,24 @@ def test_large_weights_that_pass_the_caches_by(k):
     assert torch.equal(lin.weight.grad, dw)
     lin(x).backward(dy)
     assert torch.equal(lin.weight.grad, dw + dw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(300, 1400, 16500), (129, 3970, 16400), (260, 4000, 8200), (200, 28000, 300), (140, 34000, 200), (130, 26000, 260)])
+def test_each_split_and_tile_of_mid_sized_products(m, n, k):
+    """Split 128 x 128 and 64 x 128 tiles, one round of 256 x 256 tiles that are not full: 16-bit and 32-bit outputs."""
+    import yolo_from_scratch_amd as yfs
+    x, w = _matrix(m, k, 51, torch.bfloat16), _matrix(n, k, 52)
+    wq = yfs.quantize_fp8(w)
+    xn, wn = hr.rounded(_np(x), 1, 128), wq.dequantize().double()
+    xg = torch.from_numpy(xn).to(DEV)
+    ref, mag = xg @ wn.t(), xg.abs() @ wn.abs().t()
+    inner = (96 + k / 32) * 2.0 ** -24 * mag
+    got = yfs.fp8_matmul(x, wq, out_dtype=torch.float32).double()
+    assert bool(((got - ref).abs() <= 2.0 ** -24 * (ref.abs() + inner) + inner).all())
+    # the 8-bit instruction: 2^-9 of the largest product of each block of 128
+    for k0 in range(0, k, 128):
+        inner = inner + 2.0 ** -9 * xg[:, k0:k0 + 128].abs().amax(1, keepdim=True) * wn[:, k0:k0 + 128].abs().amax(1)
+    got = yfs.fp8_matmul(x, wq).double()
+    assert bool(((got - ref).abs() <= 2.0 ** -8 * (ref.abs() + inner) + inner).all())
+    assert torch.equal(yfs.fp8_matmul(x, wq).double(), got)

@@ -905,7 +905,8 @@ constexpr int kRows = 16;              // rows that fp8_rows_kernel can take
 constexpr size_t kRowsLds = 128 * 1024;   // its quantised rows in LDS
 constexpr int kCUs = 256;
 
-struct Plan { int kind, bm, bn, splits, per_split; long long body; };   // kind 0: fp8_rows_kernel, 1: fp8_gemm_kernel, 2: fp8_gemm8_kernel
+// two: two workgroups per CU although the reduction is split; body: rows that kind 2 takes
+struct Plan { int kind, bm, bn, splits, per_split; long long body; bool two = false; };   // kind 0: fp8_rows_kernel, 1: fp8_gemm_kernel, 2: fp8_gemm8_kernel
 size_t rows_lds(long long M, int per_split) { return ((size_t)per_split * M * 129 + 15) & ~(size_t)15; }
 void set_splits(Plan& p, long long s, int kblocks) {
     if (s < 1) s = 1;
@@ -914,17 +915,23 @@ void set_splits(Plan& p, long long s, int kblocks) {
 }
 // Operands that are both in 8 bits.  The largest tile of which there are enough for the chip (measured on the sizes in
 // brackets, us, against the next best):
-//   256 x 256 from two thirds of a round of 256 on, where they are three quarters full (3000 x 4096 x 4096: 49 / 56; 2048 x 4096 x 4096, half a round: 47 / 38)
-//   128 x 128 from two workgroups per CU on (2048 x 4096 x 4096: 38 / 50)
+//   256 x 256 from two thirds of a round of 256 on, where they are three quarters full (3000 x 4096 x 4096: 49 / 56; 2048 x 4096 x 4096,
+//             half a round: 47 / 38), and where they fit one round and the next smaller do not (160 x 50176 x 4096: 61 / 87)
+//   128 x 128 from three workgroups on two CUs on (300 x 16384 x 4096: 31 / 34; 1024 x 4096 x 8192, one per CU: 47 / 41); with fp32
+//             sums, from seven on four (1470 x 4096 x 2009, three on two: 33 / 31)
 //   64 x 128  from one per CU on (2048 x 2048 x 2048: 16 / 18; 64 x 50176 x 4096: 48 / 56)
-//   64 x 64   from three quarters of that on (300 x 4096 x 4096: 17 / 21)
-//   else 64 x 128 with the reduction split until there is one per CU, 4 blocks or more each (64 x 4096 x 50176: 44 / 47)
+// Fewer, and the reduction is split, 4 blocks or more each (more parts than these cost more in the join than they bring):
+//   128 blocks or more: 128 x 128 with three stages, one per CU, up to 8 parts, where that leaves less than a quarter of the CUs
+//             (128 x 4096 x 50176: 52 / 62; 2000 x 500 x 20000: 36 / 59; 100 x 300 x 50000, 79 parts: 20 / 16)
+//   64 blocks or more: 64 x 128, two per CU, up to 8 parts (300 x 4096 x 16384: 37 / 57; 193 x 1678 x 10146, 9 parts: 25 / 21)
+//   64 x 64 unsplit        where they are three quarters of one per CU (300 x 4096 x 4096: 17 / 21)
+//   64 x 128, one per CU   (64 x 4096 x 50176: 44 / 47)
 // `exact` (fp32 outputs): no 256 x 256 form; 8 waves on the 128 x 128 tile where the reduction is so short that the stores
 // are what counts (4096 x 50176 x 64: 139 / 157; 4096 x 4096 x 4096: 126 / 116 the other way round).
 Plan plan_tiles(long long M, long long N, int kblocks, bool exact) {
     Plan p = {1, 128, 128, 1, kblocks, 0};
-    const long long mt = yfs_cdiv(M, 256), nt = yfs_cdiv(N, 256), t256 = mt * nt;
-    if (!exact && 3 * t256 >= 2 * kCUs && 4 * M * N >= 3 * t256 * 65536) {
+    const long long mt = yfs_cdiv(M, 256), nt = yfs_cdiv(N, 256), t256 = mt * nt, t128 = yfs_cdiv(M, 128) * yfs_cdiv(N, 128);
+    if (!exact && ((3 * t256 >= 2 * kCUs && 4 * M * N >= 3 * t256 * 65536) || (t256 <= kCUs && t128 > 2 * kCUs))) {
         p.kind = 2;
         p.bm = p.bn = 256;
         // A last round of fewer than half the CUs costs as much as a full one: its tile rows go to the small tiles instead
@@ -933,15 +940,23 @@ Plan plan_tiles(long long M, long long N, int kblocks, bool exact) {
         p.body = whole * 256 < M ? whole * 256 : M;
         return p;
     }
-    if (yfs_cdiv(M, 128) * yfs_cdiv(N, 128) >= 2 * kCUs - kCUs / 4) return p;
+    if (M > 64 && 4 * t128 >= (exact ? 7 : 6) * kCUs) return p;
+    const long long deep = kCUs / t128;
+    if (kblocks >= 128 && M > 64 && deep > 1 && deep <= 8 && 4 * deep * t128 > 3 * kCUs) {
+        set_splits(p, deep < kblocks / 4 ? deep : kblocks / 4, kblocks);
+        return p;
+    }
     p.bm = 64;
     const long long wide = yfs_cdiv(M, 64) * yfs_cdiv(N, 128);
-    if (wide >= kCUs) return p;
-    if (yfs_cdiv(M, 64) * yfs_cdiv(N, 64) >= kCUs - kCUs / 4) {
+    long long s = kCUs / wide;
+    if (kblocks >= 64 && M > 64 && wide > kCUs / 4) {
+        p.two = true;
+        s = 2 * kCUs / wide;
+    } else if (wide >= kCUs) s = 1;
+    else if (yfs_cdiv(M, 64) * yfs_cdiv(N, 64) >= kCUs - kCUs / 4) {
         p.bn = 64;
         return p;
     }
-    long long s = kCUs / wide;
     if (s > kblocks / 4) s = kblocks / 4;
     set_splits(p, s, kblocks);
     return p;
@@ -1028,11 +1043,12 @@ int gemm(GemmArgs g, hipStream_t s) {
         if constexpr (EXACT) {
             if (g.kblocks <= 4) return launch_tiles<4, 2, 2, 4, 2, ROWB, EXACT, TO>(g, s);
         }
+        if (p.splits > 1) return launch_tiles<4, 2, 2, 4, 3, ROWB, EXACT, TO>(g, s);
         return launch_tiles<4, 4, 2, 2, 2, ROWB, EXACT, TO>(g, s);
     }
     if (p.bn == 64) return launch_tiles<2, 2, 2, 2, 3, ROWB, EXACT, TO>(g, s);
-    // (unsplit, four workgroups of two stages per CU; split, there is one per CU, and three stages keep more on their way)
-    if (p.splits == 1) return launch_tiles<4, 2, 1, 4, 2, ROWB, EXACT, TO>(g, s);
+    // (unsplit, four workgroups of two stages per CU; split to one per CU, three stages keep more on their way)
+    if (p.splits == 1 || p.two) return launch_tiles<4, 2, 1, 4, 2, ROWB, EXACT, TO>(g, s);
     return launch_tiles<4, 2, 1, 4, 3, ROWB, EXACT, TO>(g, s);
 }
 
