@@ -776,6 +776,8 @@ __global__ void __launch_bounds__(1024) fp8_rows_kernel(GemmArgs g, const T* x, 
 // quantised, transposed for the backward pass and multiplied while they are on the chip.  A workgroup takes 128 columns of y and
 // per_split blocks of the reduction; per block the 128 x 128 weights are read once, leave through LDS as 8-bit columns (qt, for dx),
 // and from LDS as rows into the products: a wave owns 32 columns of all 64 rows.  The partial sums are joined by fp8_join_kernel.
+// 64 x 4096 x 50176, fp32 weights: 232 us, 4.5 TB/s of 822 MB read and 222 MB written (quantiser and product one after the other: 251 + 48).
+// Three workgroups per CU, the next block's weights ahead in registers, x straight from L2: 287, 264, 275 where two plain ones took 251.
 template <typename T, typename TO>
 __global__ void __launch_bounds__(256) fp8_train_rows_kernel(GemmArgs g, QuantArgs w) {
     constexpr bool EXACT = sizeof(TO) == 4;
