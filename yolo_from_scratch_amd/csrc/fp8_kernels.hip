@@ -29,9 +29,8 @@ __host__ __device__ inline long long pad128(long long n) { return (n + 127) & ~1
 __host__ __device__ inline int groups64(long long rows) { return (int)((rows + 255) / 256 * 4); }
 __host__ __device__ inline long long packed_bytes(long long rows, long long kblocks) { return kblocks * groups64(rows) * 64; }
 
-// e of the smallest power of two with amax <= 448 * 2^e = 0.875 * 2^(e + 9); amax finite and >= 0
-__device__ __forceinline__ int scale_exponent(float amax) {
-    const unsigned u = __float_as_uint(amax);
+// e of the smallest power of two with amax <= 448 * 2^e = 0.875 * 2^(e + 9); amax finite and >= 0, given by its bits
+__device__ __forceinline__ int scale_exponent(unsigned u) {
     const int e = (int)(u >> 23) - 126 - 9 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);   // a subnormal amax ends below -127
     return u == 0 ? 0 : (e < -127 ? -127 : e);
 }
@@ -44,9 +43,42 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)
 // 184 x 4965 x 35251: 718 us, 697 through the caches; its quantiser at 184 x 4992 x 35200 the other way round, 192 against 235).
 __host__ __device__ inline bool past_caches(long long row_bytes, long long bytes) { return bytes >= (128LL << 20) && row_bytes % 128 == 0; }
 
-__device__ __forceinline__ float finite_abs(float v) {
-    const float a = fabsf(v);
-    return a < __builtin_inff() ? a : 0.0f;
+// Largest magnitudes are found among the bits, which are in the same order: one three-operand maximum takes two values.  Only a thread
+// that meets an Inf or NaN looks at its values again, one by one.
+constexpr unsigned kInfBits = 0x7F800000u;
+__device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+__device__ __forceinline__ unsigned finite_bits(float v) {
+    asm volatile("" : "+v"(v));   // (or the magnitudes of the first look are kept for this one: 62 registers more)
+    return abs_bits(v) < kInfBits ? abs_bits(v) : 0u;
+}
+template <int N>
+__device__ __forceinline__ unsigned top_bits(const float (&v)[N]) {
+    unsigned a = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) a = umax(a, abs_bits(v[j]));
+    return a;
+}
+template <int N>
+__device__ __forceinline__ unsigned finite_top(const float (&v)[N]) {
+    unsigned a = top_bits(v);
+    if (a >= kInfBits) {
+        a = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) a = umax(a, finite_bits(v[j]));
+    }
+    return a;
+}
+__device__ __forceinline__ unsigned finite_top(const float (&v)[8][8]) {
+    unsigned a = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = umax(a, top_bits(v[i]));
+    if (a >= kInfBits) {
+        a = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = umax(a, finite_top(v[i]));
+    }
+    return a;
 }
 __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
     int p = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
@@ -81,7 +113,7 @@ __device__ __forceinline__ void load_block(const QuantArgs& g, long long m, long
 // Weights: one workgroup and one scale per 128 x 128 tile, 8 x 8 elements per thread; the transpose leaves through LDS.
 template <typename T, bool COLQ>
 __global__ void __launch_bounds__(256) quant_block_kernel(QuantArgs g) {
-    __shared__ float red[4];
+    __shared__ unsigned red[4];
     __shared__ __attribute__((aligned(16))) unsigned char tile[COLQ ? 128 * 144 : 16];
     const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4, wave = threadIdx.x >> 6;
     // Neighbouring workgroups take a patch of up to 32 tiles down by the rest across: rows of a power of two times an odd number
@@ -91,17 +123,14 @@ __global__ void __launch_bounds__(256) quant_block_kernel(QuantArgs g) {
     const long long kb = in / high, mb = grp * 32 + in - (int)kb * high;
     const long long k0 = kb * 128 + cg * 8, m0 = mb * 128 + rg * 8;
     const long long ldq = pad128(g.K), ldt = pad128(g.M);
-    float v[8][8], a = 0.0f;
+    float v[8][8];
     load_block<T>(g, m0, k0, v);
+    unsigned a = finite_top(v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(v[i][j]));
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+    for (int o = 32; o > 0; o >>= 1) a = umax(a, (unsigned)__shfl_xor((int)a, o, 64));
     if ((threadIdx.x & 63) == 0) red[wave] = a;
     __syncthreads();
-    const int e = scale_exponent(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    const int e = scale_exponent(umax(umax(red[0], red[1]), umax(red[2], red[3])));
     const float f = pow2(-e);
     if (threadIdx.x == 0) {
         g.s[mb * (ldq >> 7) + kb] = (unsigned char)(e + 127);
@@ -130,26 +159,27 @@ __global__ void __launch_bounds__(256) quant_block_kernel(QuantArgs g) {
     }
 }
 
-// Activations and gradients.  The first row_blocks workgroups quantise by rows, 16 lanes x 8 elements per block, blocks of a row
+// Activations and gradients.  The last row_blocks workgroups quantise by rows, 16 lanes x 8 elements per block, blocks of a row
 // next to each other (four rows per thread, whose scales fill a dword of the packed plane, were slower: 12544 x 4096 bf16 35 us
-// against 29, 5.3 TB/s).  The others take 128 rows x 64 columns: column sums, and the transpose by rows, through LDS.  The second
-// read of x comes from the caches; one 128 x 128 tile for both took 14 us where this takes 10 (64 x 50176 bf16): too few
-// workgroups with too long a chain of reductions each.
+// against 29, 5.3 TB/s).  The others, first because each takes longer, have 128 rows x 64 columns: column sums, and the transpose by
+// rows, through LDS.  The second read of x comes from the caches; one 128 x 128 tile for both took 14 us where this takes 8
+// (64 x 50176 bf16): too few workgroups with too long a chain of reductions each.
 template <typename T>
 __global__ void __launch_bounds__(256) quant_rows_kernel(QuantArgs g) {
-    __shared__ float top[4][64], sum[4][64];
+    __shared__ unsigned top[4][64];
+    __shared__ float sum[4][64];
     __shared__ unsigned tile[64 * 33];   // [column][128 rows + 4 bytes]
-    if ((int)blockIdx.x < g.row_blocks) {
+    const int col_blocks = (int)gridDim.x - g.row_blocks;
+    if ((int)blockIdx.x >= col_blocks) {
         const long long kblocks = (g.K + 127) >> 7, total = g.M * kblocks;
         const int l = threadIdx.x & 15;
-        for (long long id = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); id < total; id += (long long)g.row_blocks * 16) {
-            const long long m = id / kblocks, kb = id - m * kblocks, k = kb * 128 + l * 8;
-            float v[8], a = 0.0f;
+        for (long long id = (long long)((int)blockIdx.x - col_blocks) * 16 + (threadIdx.x >> 4); id < total; id += (long long)g.row_blocks * 16) {
+            const long long m = total >> 32 ? id / kblocks : (unsigned)id / (unsigned)kblocks, kb = id - m * kblocks, k = kb * 128 + l * 8;
+            float v[8];
             load_vec8((const T*)g.x + m * g.ld + k, g.K - k, v);
+            unsigned a = finite_top(v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(v[j]));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+            for (int o = 8; o > 0; o >>= 1) a = umax(a, (unsigned)__shfl_xor((int)a, o, 64));
             const int e = scale_exponent(a);
             if (l == 0) g.s[(kb * g.groups + (m >> 6)) * 64 + (m & 15) * 4 + ((m & 63) >> 4)] = (unsigned char)(e + 127);
             const float f = pow2(-e);
@@ -158,27 +188,39 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(QuantArgs g) {
         }
         return;
     }
-    const long long strips = (g.K + 63) >> 6, id = (long long)blockIdx.x - g.row_blocks, mb = id / strips, strip = id - mb * strips, k0 = strip * 64;
+    const unsigned strips = (unsigned)((g.K + 63) >> 6);
+    const long long mb = blockIdx.x / strips, strip = blockIdx.x - (unsigned)mb * strips, k0 = strip * 64;
     const int cg = threadIdx.x & 7, rg = threadIdx.x >> 3, wave = threadIdx.x >> 6;
     const long long m0 = mb * 128 + rg * 4, kc = k0 + cg * 8, ldt = pad128(g.M);
     float v[4][8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) load_vec8((const T*)g.x + (m0 + i) * g.ld + kc, m0 + i < g.M ? g.K - kc : 0, v[i]);
+    unsigned a[8], all = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        float a = 0.0f, s = 0.0f;
+        a[j] = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a = fmaxf(a, finite_abs(v[i][j]));
-            s += v[i][j];
+        for (int i = 0; i < 4; ++i) a[j] = umax(a[j], abs_bits(v[i][j]));
+        all = umax(all, a[j]);
+    }
+    if (all >= kInfBits) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            a[j] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[j] = umax(a[j], finite_bits(v[i][j]));
         }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float s = (v[0][j] + v[1][j]) + (v[2][j] + v[3][j]);
 #pragma unroll
         for (int o = 8; o < 64; o <<= 1) {
-            a = fmaxf(a, __shfl_xor(a, o, 64));
+            a[j] = umax(a[j], (unsigned)__shfl_xor((int)a[j], o, 64));
             if (g.colsum) s += __shfl_xor(s, o, 64);
         }
         if ((threadIdx.x & 56) == 0) {
-            top[wave][cg * 8 + j] = a;
+            top[wave][cg * 8 + j] = a[j];
             sum[wave][cg * 8 + j] = s;
         }
     }
@@ -186,7 +228,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(QuantArgs g) {
     if (g.colsum && threadIdx.x < 64 && k0 + threadIdx.x < g.K)
         g.colsum[mb * g.K + k0 + threadIdx.x] = (sum[0][threadIdx.x] + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x]);
     if (!g.qt) return;
-    auto exponent = [&](int c) { return scale_exponent(fmaxf(fmaxf(top[0][c], top[1][c]), fmaxf(top[2][c], top[3][c]))); };
+    auto exponent = [&](int c) { return scale_exponent(umax(umax(top[0][c], top[1][c]), umax(top[2][c], top[3][c]))); };
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float f = pow2(-exponent(cg * 8 + j));
@@ -739,12 +781,11 @@ __global__ void __launch_bounds__(1024) fp8_rows_kernel(GemmArgs g, const T* x, 
         for (int id = (int)(threadIdx.x >> 4); id < nkb * rows; id += groups) {
             const int blk = id / rows, m = id - blk * rows;
             const long long k = (long long)(kb0 + blk) * 128 + l * 8;
-            float v[8], top = 0.0f;
+            float v[8];
             load_vec8(x + m * ldx + k, K - k, v);
+            unsigned top = finite_top(v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(v[j]));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+            for (int o = 8; o > 0; o >>= 1) top = umax(top, (unsigned)__shfl_xor((int)top, o, 64));
             const int e = scale_exponent(top);
             const float f = pow2(-e);
             *reinterpret_cast<uint2*>(smem + (long long)id * 128 + l * 8) =
@@ -781,7 +822,7 @@ __global__ void __launch_bounds__(1024) fp8_rows_kernel(GemmArgs g, const T* x, 
 template <typename T, typename TO>
 __global__ void __launch_bounds__(256) fp8_train_rows_kernel(GemmArgs g, QuantArgs w) {
     constexpr bool EXACT = sizeof(TO) == 4;
-    __shared__ float red[4];
+    __shared__ unsigned red[4];
     __shared__ __attribute__((aligned(16))) unsigned char wt[128 * 128], xt[64 * 128], tt[128 * 144];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, frow = lane & 15, fk = lane >> 4;
     const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4;
@@ -798,7 +839,7 @@ __global__ void __launch_bounds__(256) fp8_train_rows_kernel(GemmArgs g, QuantAr
     for (int i = 0; i < 8; ++i) (&acc[0][0])[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
     for (int kb = kb0; kb < kb1; ++kb) {
         const long long k0 = kb * 128LL + cg * 8;
-        float v[8][8], a = 0.0f;
+        float v[8][8];
         load_block<T>(w, m0, k0, v);
         i32x4 xv[2];
 #pragma unroll
@@ -808,15 +849,12 @@ __global__ void __launch_bounds__(256) fp8_train_rows_kernel(GemmArgs g, QuantAr
             if (row < g.M) xv[i] = *reinterpret_cast<const i32x4*>(g.a + row * ldx + kb * 128LL + (threadIdx.x & 7) * 16);
         }
         const int sa = *reinterpret_cast<const int*>(g.as + (long long)kb * g.groups_a * 64 + frow * 4);
+        unsigned a = finite_top(v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_abs(v[i][j]));
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+        for (int o = 32; o > 0; o >>= 1) a = umax(a, (unsigned)__shfl_xor((int)a, o, 64));
         if (lane == 0) red[wave] = a;
         __syncthreads();   // (and every wave has left the block before this one)
-        const int e = scale_exponent(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+        const int e = scale_exponent(umax(umax(red[0], red[1]), umax(red[2], red[3])));
         const float f = pow2(-e);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
