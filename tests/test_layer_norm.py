@@ -399,3 +399,31 @@ def test_longest_row():
     dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
     assert torch.equal(dx, dy) and torch.equal(db, dy[0].float())
     assert float((dw - dy[0].float() * x[0].detach().float()).abs().max()) <= 32 * 2.0 ** -24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(5, 8200), (3, 16384), (4, 16392), (3, 20001), (2, 32761), (2, 36693), (2, 50177), (2, 65536), (2, 65543), (1030, 8200),
+                                       (1025, 12001), (1100, 16384)])
+def test_rows_kept_in_their_own_type(rows, cols, dtype):
+    """Widths on both sides of each form of the long rows' kernels, whole vectors and not, with and without sums in the pass of dx."""
+    import yolo_from_scratch_amd as yfs
+    x, w, b, dy = _inputs(rows, cols, DTYPES[dtype])
+    for v in (x, w, b):
+        v.requires_grad_()
+    y = yfs.layer_norm(x, w, b)
+    got = torch.autograd.grad(y, (x, w, b), dy)
+    if rows > 1000:     # the sums in 64 bits of the whole columns, the rest of a few rows
+        xs, wd, dd = x.detach().double(), w.detach().double(), dy.double()
+        h = (xs - xs.mean(1, keepdim=True)) / torch.sqrt(xs.var(1, unbiased=False, keepdim=True) + 1e-5)
+        tol = (len(xs) + 256) * 2.0 ** -24 * (dd * h).abs().sum(0) + 2 * 8 * K * dd.abs().sum(0)
+        assert bool(((got[1].double() - (dd * h).sum(0)).abs() <= tol).all())
+        assert bool(((got[2].double() - dd.sum(0)).abs() <= (len(xs) + 256) * 2.0 ** -24 * dd.abs().sum(0)).all())
+        pick = [0, 1, rows // 2, rows - 1]
+        _check_forward(_np(y[pick]), _np(x[pick]), _np(w), _np(b), 1e-5, x.dtype)
+        _check_backward(_np(got[0][pick]), None, None, _np(dy[pick]), _np(x[pick]), _np(w), 1e-5, x.dtype)
+        return
+    _check_forward(_np(y), _np(x), _np(w), _np(b), 1e-5, x.dtype)
+    _check_backward(*[_np(v) for v in got], _np(dy), _np(x), _np(w), 1e-5, x.dtype)
+    only = torch.autograd.grad(yfs.layer_norm(x, w.detach(), b.detach()), x, dy)[0]
+    assert torch.equal(only, got[0])

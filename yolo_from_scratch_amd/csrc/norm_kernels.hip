@@ -109,6 +109,79 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) ln_fwd_kernel(const T* __re
     }
 }
 
+// Weights of a thread's vectors, the next one's on their way while one is used: all at once would take the registers of the row itself
+template <int VE>
+struct Ahead {
+    const float* p;
+    int cols;
+    float none, v[2][VE];
+    __device__ __forceinline__ void fetch(int i, int at, int c) { load_vec_or(p ? p + at : p, c, cols - at, v[i & 1], none); }
+};
+__device__ __forceinline__ void no_loads_earlier() { asm volatile("" ::: "memory"); }
+
+// Rows of more than 2048 vectors, up to 8192: one workgroup of up to 16 waves per row, NV vectors per thread, kept in their own type
+// between the passes (an fp32 copy would be twice the registers of a 16-bit row and leave one workgroup per CU); weight and bias come
+// from L2.
+template <typename T, int NV, bool ODD>
+__global__ void __launch_bounds__(1024) ln_fwd_wide_kernel(const T* __restrict__ x, long long xs, const float* __restrict__ w,
+                                                           const float* __restrict__ b, T* __restrict__ y, float* __restrict__ mean,
+                                                           float* __restrict__ rstd, long long rows, int cols, float eps) {
+    constexpr int VE = 16 / sizeof(T);
+    __shared__ float2 red[32];
+    const int G = (int)blockDim.x, step = G * VE, c = (int)threadIdx.x * VE;   // vector i of the thread: i * step + c
+    bool whole[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) whole[i] = ODD && __all(i * step + c + VE <= cols);
+    const float inv = 1.0f / (float)cols;
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        yfs_int4 raw[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) raw[i] = load_raw<ODD>(x + row * xs + i * step, c, cols - i * step, whole[i]);
+        float s = 0.0f, q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float v[VE];
+            widen_raw<T>(raw[i], v);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) s += v[j];
+        }
+        const float mu = row_sum<true>(s, 0.0f, G, red, 0).x * inv;
+        fence(raw);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float v[VE];
+            widen_raw<T>(raw[i], v);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                const float d = v[j] - mu;
+                q += (ODD ? whole[i] || c + j < cols - i * step : c < cols - i * step) ? d * d : 0.0f;
+            }
+        }
+        const float r = 1.0f / sqrtf(row_sum<true>(q, 0.0f, G, red, 1).x * inv + eps);
+        fence(raw);
+        if (c == 0) {
+            if (mean) mean[row] = mu;
+            if (rstd) rstd[row] = r;
+        }
+        Ahead<VE> pw = {w, cols, 1.0f}, pb = {b, cols, 0.0f};
+        pw.fetch(0, 0, c);
+        pb.fetch(0, 0, c);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (i + 1 < NV) {
+                pw.fetch(i + 1, (i + 1) * step, c);
+                pb.fetch(i + 1, (i + 1) * step, c);
+                no_loads_earlier();
+            }
+            float v[VE];
+            widen_raw<T>(raw[i], v);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) v[j] = (v[j] - mu) * r * pw.v[i & 1][j] + pb.v[i & 1][j];
+            store_row<ODD>(y + row * cols + i * step, c, cols - i * step, whole[i], v);
+        }
+    }
+}
+
 // Rows longer than a workgroup's registers: the row is read three times (the second and third time from L2).
 template <typename T>
 __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(const T* __restrict__ x, long long xs, const float* __restrict__ w,
@@ -306,6 +379,93 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256) ln_bwd_kernel(BwdArgs g) {
     }
 }
 
+// Rows of more than 1024 vectors, up to 4096 (eight of x and of dy per thread do not fit).  ACC: with the sums of dw and db, in workgroups
+// of up to 512 (2000 x 16384 bf16: 63 us, with column sums by other workgroups 80).  fp32 rows fit five waves a SIMD: 2500 x 9000
+// 92 us against 131 with four.
+template <typename T, int NV, bool ACC, bool ODD>
+__global__ void __launch_bounds__(ACC ? 512 : 1024, ACC ? 1 : (sizeof(T) == 4 ? 5 : 4)) ln_bwd_wide_kernel(BwdArgs g) {
+    constexpr int VE = 16 / sizeof(T);
+    __shared__ float2 red[32];
+    extern __shared__ float sums[];
+    if (!ACC && (int)blockIdx.x >= g.dx_blocks) {
+        column_sums<T>(g, (int)blockIdx.x - g.dx_blocks, sums);
+        return;
+    }
+    const int G = (int)blockDim.x, step = G * VE, c = (int)threadIdx.x * VE;
+    bool whole[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) whole[i] = ODD && __all(i * step + c + VE <= g.cols);
+    const float inv = 1.0f / (float)g.cols;
+    float aw[ACC ? NV : 1][VE], ab[ACC ? NV : 1][VE];
+    if (ACC) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VE; ++j) aw[i][j] = ab[i][j] = 0.0f;
+    }
+    int slot = 0;
+    for (long long row = blockIdx.x; row < g.rows; row += g.dx_blocks) {
+        const float mu = g.mean[row], r = g.rstd[row];
+        yfs_int4 xr[NV], dr[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            xr[i] = load_raw<ODD>((const T*)g.x + row * g.xs + i * step, c, g.cols - i * step, whole[i]);
+            dr[i] = load_raw<ODD>((const T*)g.dy + row * g.dys + i * step, c, g.cols - i * step, whole[i]);
+        }
+        float s1 = 0.0f, s2 = 0.0f;
+        Ahead<VE> pw = {g.w, g.cols, 1.0f};
+        pw.fetch(0, 0, c);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (i + 1 < NV) {
+                pw.fetch(i + 1, (i + 1) * step, c);
+                no_loads_earlier();
+            }
+            const float (&wv)[VE] = pw.v[i & 1];
+            float xv[VE], dv[VE];
+            widen_raw<T>(xr[i], xv);
+            widen_raw<T>(dr[i], dv);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {   // (dy is 0 behind the row)
+                const float h = (ODD ? whole[i] || c + j < g.cols - i * step : c < g.cols - i * step) ? (xv[j] - mu) * r : 0.0f, d = dv[j];
+                if (ACC) {
+                    aw[i][j] += d * h;
+                    ab[i][j] += d;
+                }
+                s1 += d * wv[j];
+                s2 += d * wv[j] * h;
+            }
+        }
+        const float2 s = row_sum<true>(s1, s2, G, red, slot);
+        slot ^= 1;
+        const float m1 = s.x * inv, m2 = s.y * inv;
+        fence(xr);
+        fence(dr);
+        pw.fetch(0, 0, c);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (i + 1 < NV) {
+                pw.fetch(i + 1, (i + 1) * step, c);
+                no_loads_earlier();
+            }
+            const float (&wv)[VE] = pw.v[i & 1];
+            float xv[VE], dv[VE];
+            widen_raw<T>(xr[i], xv);
+            widen_raw<T>(dr[i], dv);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) dv[j] = r * (dv[j] * wv[j] - m1 - (xv[j] - mu) * r * m2);
+            store_row<ODD>((T*)g.dx + row * g.cols + i * step, c, g.cols - i * step, whole[i], dv);
+        }
+    }
+    if constexpr (ACC) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            store_vec(g.dw + (long long)blockIdx.x * 2 * g.cols + i * step + c, g.cols - i * step - c, aw[i]);
+            store_vec(g.db + (long long)blockIdx.x * 2 * g.cols + i * step + c, g.cols - i * step - c, ab[i]);
+        }
+    }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(1024) ln_bwd_long_kernel(BwdArgs g) {
     constexpr int VE = 16 / sizeof(T);
@@ -369,18 +529,23 @@ __global__ void __launch_bounds__(1024) ln_reduce_kernel(const float* __restrict
 }
 
 constexpr int kCUs = 256;
-struct Shape { int nv, lg, threads; };   // lg >= 0: groups of 2^lg lanes; lg < 0: one workgroup per row; nv == 0: the long form
+// lg >= 0: groups of 2^lg lanes; lg < 0: one workgroup per row; nv == 0: the long form
+struct Shape { int nv, lg, threads; bool wide = false; };
 // A wave per row up to `wave_most` vectors a lane (three, with dw and db summed, are 186 registers: 1470 bf16 columns 160 us against
 // 126 in workgroups of 128, 50000 rows backward; without sums three fit: 74 against 85 forward).  Longer rows have two vectors per
-// thread (4096 bf16 columns: 43 us against 49 with one, 12544 rows forward), up to `most` in a workgroup of 512.
-Shape ln_shape(int cols, int esize, int wave_most, int most) {
+// thread (4096 bf16 columns: 43 us against 49 with one, 12544 rows forward), `block_most` in a workgroup of 512, and the wide kernels'
+// four or eight (`wide_most`) in one of up to 1024 (forward, with four: 3000 x 12000 bf16 45 us against 52 in the wide form, which takes
+// 2500 x 20000 in 72 us where three readings of the row take 135; backward, 104 in the wide form against 139).
+Shape ln_shape(int cols, int esize, int wave_most, int block_most, int wide_most) {
     const long long vecs = yfs_cdiv(cols, 16 / esize);
     for (int lg = 3; lg <= 6; ++lg)
         if (vecs <= (1 << lg)) return {1, lg, 256};
     for (int nv = 2; nv <= wave_most; ++nv)
         if (vecs <= 64 * nv) return {nv, 6, 256};
-    for (int nv = 2; nv <= most; nv *= 2)
-        if (vecs <= 512LL * nv) return {nv, -1, (int)(yfs_cdiv(vecs, 64 * nv) * 64)};
+    for (int nv = 2; nv <= block_most; nv *= 2)
+        if (vecs <= 512 * nv) return {nv, -1, (int)(yfs_cdiv(vecs, 64 * nv) * 64)};
+    for (int nv = 4; nv <= wide_most; nv *= 2)
+        if (vecs <= 1024 * nv) return {nv, -1, (int)(yfs_cdiv(vecs, 64 * nv) * 64), true};
     return {0, -1, 1024};
 }
 // Workgroups that take the rows in turn: 32 waves a CU where a wave has a row, 16 where a workgroup has one
@@ -394,14 +559,15 @@ unsigned row_blocks(long long rows, const Shape& s) {
 struct BwdPlan { Shape sh; bool acc; int dx_blocks, strips, parts; long long part_rows; };
 BwdPlan bwd_plan(long long rows, int cols, int esize, bool need_dx) {
     BwdPlan p;
-    p.sh = ln_shape(cols, esize, 2, 4);
-    p.dx_blocks = need_dx ? (int)row_blocks(rows, p.sh) : 0;
+    p.sh = ln_shape(cols, esize, 2, 2, 4);
     p.strips = (int)yfs_cdiv(cols, 32 * (16 / esize));
     const long long rpb = p.sh.lg >= 0 ? 256 >> p.sh.lg : 1;
     // a partial sum is 8 bytes a column, written and read, a row of x, dy and dx 6 or 12: from 4 rows a workgroup on it is less than
     // reading x and dy again
-    const long long fill = kCUs * 16 * 64 / p.sh.threads, nb = rows / (rpb * 4);   // 16 waves per CU
-    p.acc = need_dx && p.sh.nv > 0 && p.sh.nv <= 2 && nb >= kCUs;
+    const long long nb = rows / (rpb * 4), vecs = yfs_cdiv(cols, 16 / esize);
+    p.acc = need_dx && vecs <= 2048 && nb >= kCUs;
+    const long long fill = kCUs * (p.sh.wide ? 8 : 16) * 64 / p.sh.threads;   // 16 waves per CU, 8 of the wide form
+    p.dx_blocks = need_dx ? (int)row_blocks(rows, p.sh) : 0;
     if (p.acc) {
         p.dx_blocks = (int)(nb < fill ? nb : fill);
         p.parts = p.dx_blocks;
@@ -421,12 +587,17 @@ template <typename T>
 int fwd(const void* x, long long xs, const float* w, const float* b, void* y, float* mean, float* rstd, long long rows, int cols,
         float eps, hipStream_t s) {
     const bool odd = cols % (16 / (int)sizeof(T)) != 0;
-    const Shape sh = ln_shape(cols, sizeof(T), 3, sizeof(T) == 2 ? 4 : 8);
+    const Shape sh = ln_shape(cols, sizeof(T), 3, 4, 8);
     const dim3 grid(row_blocks(rows, sh)), blk(sh.threads);
 #define LN_FWD(NV, BLOCK)                                                                                                              \
     do {                                                                                                                               \
         if (odd) ln_fwd_kernel<T, NV, BLOCK, true><<<grid, blk, 0, s>>>((const T*)x, xs, w, b, (T*)y, mean, rstd, rows, cols, eps, sh.lg);   \
         else ln_fwd_kernel<T, NV, BLOCK, false><<<grid, blk, 0, s>>>((const T*)x, xs, w, b, (T*)y, mean, rstd, rows, cols, eps, sh.lg);       \
+    } while (0)
+#define LN_WIDE(NV)                                                                                                                \
+    do {                                                                                                                             \
+        if (odd) ln_fwd_wide_kernel<T, NV, true><<<grid, blk, 0, s>>>((const T*)x, xs, w, b, (T*)y, mean, rstd, rows, cols, eps);      \
+        else ln_fwd_wide_kernel<T, NV, false><<<grid, blk, 0, s>>>((const T*)x, xs, w, b, (T*)y, mean, rstd, rows, cols, eps);          \
     } while (0)
     if (sh.nv == 0)
         ln_fwd_long_kernel<T><<<grid, blk, 0, s>>>((const T*)x, xs, w, b, (T*)y, mean, rstd, rows, cols, eps);
@@ -434,11 +605,12 @@ int fwd(const void* x, long long xs, const float* w, const float* b, void* y, fl
         if (sh.nv == 1) LN_FWD(1, false);
         else if (sh.nv == 2) LN_FWD(2, false);
         else LN_FWD(3, false);
+    } else if (sh.wide) {
+        if (sh.nv == 4) LN_WIDE(4);
+        else LN_WIDE(8);
     } else if (sh.nv == 2) LN_FWD(2, true);
-    else if (sh.nv == 4) LN_FWD(4, true);
-    else {
-        if constexpr (sizeof(T) == 4) LN_FWD(8, true);
-    }
+    else LN_FWD(4, true);
+#undef LN_WIDE
 #undef LN_FWD
     YFS_CHECK_LAUNCH("ln_fwd_kernel");
     return YFS_OK;
@@ -470,15 +642,22 @@ int bwd(BwdArgs g, float* part, hipStream_t s) {
                              : (sums ? (size_t)p.sh.threads / 64 * 2 * 32 * (16 / sizeof(T)) * sizeof(float) : 0);
 #define LN_BWD(NV, BLOCK, ACC) \
     do { if (odd) ln_bwd_kernel<T, NV, BLOCK, ACC, true><<<grid, blk, lds, s>>>(g); else ln_bwd_kernel<T, NV, BLOCK, ACC, false><<<grid, blk, lds, s>>>(g); } while (0)
+#define LN_WIDE(NV, ACC) \
+    do { if (odd) ln_bwd_wide_kernel<T, NV, ACC, true><<<grid, blk, lds, s>>>(g); else ln_bwd_wide_kernel<T, NV, ACC, false><<<grid, blk, lds, s>>>(g); } while (0)
     if (p.sh.nv == 0) ln_bwd_long_kernel<T><<<grid, blk, lds, s>>>(g);
     else if (p.sh.lg >= 0) {
         if (p.sh.nv == 1 && p.acc) LN_BWD(1, false, true);
         else if (p.sh.nv == 1) LN_BWD(1, false, false);
         else if (p.acc) LN_BWD(2, false, true);
         else LN_BWD(2, false, false);
-    } else if (p.sh.nv == 4) LN_BWD(4, true, false);
-    else if (p.acc) LN_BWD(2, true, true);
-    else LN_BWD(2, true, false);
+    } else if (p.sh.nv == 2) {
+        if (p.acc) LN_BWD(2, true, true);
+        else LN_BWD(2, true, false);
+    } else {
+        if (p.acc) LN_WIDE(4, true);
+        else LN_WIDE(4, false);
+    }
+#undef LN_WIDE
 #undef LN_BWD
     YFS_CHECK_LAUNCH("ln_bwd_kernel");
     if (sums && join) {

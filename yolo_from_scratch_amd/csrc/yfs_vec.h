@@ -100,3 +100,32 @@ __device__ __forceinline__ void load_vec8_once(const T* p, long long n, float (&
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = (float)t[j];
 }
+
+// 16 bytes of a row as they lie in memory: what a kernel keeps in registers between two passes over a long row.  fence() before the
+// second pass, or the widened values of the first are kept instead, twice the registers of a 16-bit row.
+typedef __attribute__((ext_vector_type(4))) int yfs_int4;
+template <bool ODD, typename T>
+__device__ __forceinline__ yfs_int4 load_raw(const T* row, int c, int n, bool whole) {
+    constexpr int VE = 16 / sizeof(T);
+    yfs_int4 r = {0, 0, 0, 0};
+    if ((ODD && whole) || (ODD ? c + VE <= n : c < n)) __builtin_memcpy(&r, row + c, 16);
+    else if (ODD && c < n) {
+        T t[VE];
+#pragma unroll
+        for (int j = 0; j < VE; ++j) t[j] = c + j < n ? row[c + j] : (T)0.0f;
+        __builtin_memcpy(&r, t, 16);
+    }
+    return r;
+}
+template <typename T, int VE = 16 / (int)sizeof(T)>
+__device__ __forceinline__ void widen_raw(const yfs_int4& r, float (&v)[VE]) {
+    T t[VE];
+    __builtin_memcpy(t, &r, 16);
+#pragma unroll
+    for (int j = 0; j < VE; ++j) v[j] = (float)t[j];
+}
+template <int N>
+__device__ __forceinline__ void fence(yfs_int4 (&r)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(r[i]));
+}
