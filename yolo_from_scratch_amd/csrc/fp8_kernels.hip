@@ -41,7 +41,8 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)
 // weights read past it), and as many bytes of gradients left in it are written back while the next kernels run (the quantiser behind
 // them 251 us, 217).  Only where rows begin on a line: elsewhere parts of lines are fetched or written twice (a training step at
 // 184 x 4965 x 35251: 718 us, 697 through the caches; its quantiser at 184 x 4992 x 35200 the other way round, 192 against 235).
-__host__ __device__ inline bool past_caches(long long row_bytes, long long bytes) { return bytes >= (128LL << 20) && row_bytes % 128 == 0; }
+constexpr long long kPastCaches = 128LL << 20;
+__host__ __device__ inline bool past_caches(long long row_bytes, long long bytes) { return bytes >= kPastCaches && row_bytes % 128 == 0; }
 
 // Largest magnitudes are found among the bits, which are in the same order: one three-operand maximum takes two values.  Only a thread
 // that meets an Inf or NaN looks at its values again, one by one.
@@ -428,7 +429,19 @@ __global__ void __launch_bounds__(64 * WM * WN) fp8_gemm_kernel(GemmArgs g) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int wm = wave / WN, wn = wave % WN;
-    const long long m0 = (long long)blockIdx.y * BM, n0 = (long long)blockIdx.x * BN;
+    int tm = (int)blockIdx.y, tn = (int)blockIdx.x;
+    if constexpr (sizeof(TO) == 4) {
+        // Workgroups go round the 8 XCDs.  Where the rows of a large output begin inside a line, neighbouring tiles share lines: each XCD then
+        // takes tiles that are neighbours (4001 x 50001 x 64: 194 us against 267; whole lines, 4096 x 50176 x 64, 159 against 139)
+        if (g.splits == 1 && g.N % 32 != 0 && g.M * g.N * 4 >= kPastCaches) {
+            const int across = (int)gridDim.x, total = across * (int)gridDim.y, lin = tm * across + tn;
+            const int q8 = total >> 3, r8 = total & 7, xcd = lin & 7;
+            const int id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (lin >> 3);
+            tm = id / across;
+            tn = id - tm * across;
+        }
+    }
+    const long long m0 = (long long)tm * BM, n0 = (long long)tn * BN;
     const long long ld = (long long)g.kblocks * 128;
     const int kb0 = (int)blockIdx.z * g.per_split;
     const int kb1 = kb0 + g.per_split < g.kblocks ? kb0 + g.per_split : g.kblocks;
