@@ -376,6 +376,10 @@ size_t yfs_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int yfs_fp8_gemm(const void *aq, const void *a_scale, const void *bq, const void *b_scale, int b_row_scales, const float *bias,
                  void *out, int out_dtype, int64_t M, int64_t N, int64_t K, float slope, int accumulate, void *workspace,
                  size_t workspace_bytes, void *stream);
+/* Dispatch query, on the host: how yfs_fp8_gemm goes over a product.  plan = {tile rows, tile columns, parts of the reduction,
+ * blocks of 128 per part, leading rows that the 256 x 256 kernel takes (the rows behind them go to smaller tiles)}. */
+enum { YFS_FP8_PLAN_LEN = 5 };
+int yfs_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int out_dtype, int64_t *plan);
 /* A linear layer's training step, w [N, K] quantised in the call: y = Q(x) Q(w)^T + bias; dx = Q(dy) Q(w), dw (+)= Q(dy^T)
  * Q(x^T)^T, db (+)= sum over rows of dy.  `needs`: which gradients the backward pass will be asked for (the same value in
  * both calls; db alone needs no product: sum dy).  `saved` (256-byte aligned, like the workspaces) goes from the forward to

@@ -618,3 +618,75 @@ def test_each_split_and_tile_of_mid_sized_products(m, n, k):
     got = yfs.fp8_matmul(x, wq).double()
     assert bool(((got - ref).abs() <= 2.0 ** -8 * (ref.abs() + inner) + inner).all())
     assert torch.equal(yfs.fp8_matmul(x, wq).double(), got)
+
+
+def _plan(m, n, k, dtype):
+    import ctypes
+    import yolo_from_scratch_amd as y
+    from yolo_from_scratch_amd import _lib as L
+    plan = (ctypes.c_int64 * 5)()
+    assert y.lib().yfs_fp8_gemm_plan(m, n, k, L.DTYPES[dtype], ctypes.addressof(plan)) == 0
+    return tuple(plan)
+
+
+def test_plan_covers_every_product():
+    """Every launch that a plan stands for has workgroups: 256 x 256 tiles have rows to take wherever they are chosen, in whole
+    tiles or to the end, and every part of a split reduction has blocks."""
+    import random
+    rng = random.Random(7)
+    size = lambda top: max(1, min(top, int(2 ** rng.uniform(0, np.log2(top + 1)))))   # noqa: E731
+    cases = [(size(1 << 15), size(1 << 18), size(1 << 17)) for _ in range(20000)]
+    # one row of 256-wide tiles in one round and a bit more
+    cases += [(m, n, k) for m in (192, 193, 200, 255, 256, 257) for n in (65536, 65537, 66000, 76800, 82944, 98304, 98305, 131072, 131073, 152064, 163840)
+              for k in (64, 4096)]
+    for m, n, k in cases:
+        for t in (torch.bfloat16, torch.float32):
+            bm, bn, parts, per, body = _plan(m, n, k, t)
+            blocks = -(-k // 128)
+            assert (bm, bn) in ((256, 256), (128, 128), (64, 128), (64, 64)), (m, n, k)
+            assert parts >= 1 and (parts - 1) * per < blocks <= parts * per, (m, n, k)
+            if bm == 256:
+                assert t != torch.float32 and parts == 1 and (0 < body < m and body % 256 == 0 or body == m), (m, n, k, body)
+            else:
+                assert body == 0
+
+
+def test_plan_refusals():
+    import yolo_from_scratch_amd as y
+    lib, p = y.lib(), 4096
+    assert lib.yfs_fp8_gemm_plan(8, 8, 8, 1, None) == -1 and lib.yfs_fp8_gemm_plan(0, 8, 8, 1, p) == -1
+    assert lib.yfs_fp8_gemm_plan(8, 8, 8, 7, p) == -2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(256, 66000, 300), (200, 82944, 130), (193, 65537, 64), (256, 131073, 140)])
+def test_one_row_of_tiles_wider_than_the_whole_rounds(m, n, k):
+    import yolo_from_scratch_amd as yfs
+    x, w = _matrix(m, k, 61, torch.bfloat16), _matrix(n, k, 62)
+    wq = yfs.quantize_fp8(w)
+    xg, wn = torch.from_numpy(hr.rounded(_np(x), 1, 128)).to(DEV), wq.dequantize().double()
+    ref = xg @ wn.t()
+    inner = (96 + k / 32) * 2.0 ** -24 * (xg.abs() @ wn.abs().t())
+    for k0 in range(0, k, 128):       # the 8-bit instruction: 2^-9 of the largest product of each block of 128
+        inner = inner + 2.0 ** -9 * xg[:, k0:k0 + 128].abs().amax(1, keepdim=True) * wn[:, k0:k0 + 128].abs().amax(1)
+    got = yfs.fp8_matmul(x, wq).double()
+    assert bool(((got - ref).abs() <= 2.0 ** -8 * (ref.abs() + inner) + inner).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [193, 200, 256])
+def test_gradients_of_a_layer_with_more_than_65536_inputs(m):
+    """dx of the head's first layer at 576 x 576 images: 82944 inputs."""
+    import yolo_from_scratch_amd as yfs
+    n, k = 130, 82944
+    x = _matrix(m, k, 63, torch.bfloat16).requires_grad_()
+    w = _matrix(n, k, 64).requires_grad_()
+    dy = _matrix(m, n, 65, torch.bfloat16)
+    dx, dw = torch.autograd.grad(yfs.fp8_linear(x, w), (x, w), dy)
+    assert torch.isfinite(dw).all()
+    dq, wq = torch.from_numpy(hr.rounded(_np(dy), 1, 128)).to(DEV), yfs.quantize_fp8(w).dequantize().double()
+    ref = dq @ wq
+    inner = (96 + n / 32) * 2.0 ** -24 * (dq.abs() @ wq.abs())
+    for n0 in range(0, n, 128):
+        inner = inner + 2.0 ** -9 * dq[:, n0:n0 + 128].abs().amax(1, keepdim=True) * wq[n0:n0 + 128].abs().amax(0)
+    assert bool(((dx.double() - ref).abs() <= 2.0 ** -8 * (ref.abs() + inner) + inner).all())

@@ -48,6 +48,7 @@ _SIGNATURES = {
     "yfs_fp8_quantize_rows": "pil" "ll" "pppp" "p" "p",
     "yfs_fp8_gemm_workspace_bytes": "lll",
     "yfs_fp8_gemm": "pppp" "i" "p" "pi" "lll" "fi" "pz" "p",
+    "yfs_fp8_gemm_plan": "llli" "p",
     "yfs_fp8_matmul_workspace_bytes": "lll",
     "yfs_fp8_matmul": "pil" "pp" "p" "pi" "lll" "f" "pz" "p",
     "yfs_fp8_linear_saved_bytes": "llli",

@@ -987,9 +987,10 @@ Plan plan_tiles(long long M, long long N, int kblocks, bool exact) {
     if (!exact && ((3 * t256 >= 2 * kCUs && 4 * M * N >= 3 * t256 * 65536) || (t256 <= kCUs && t128 > 2 * kCUs))) {
         p.kind = 2;
         p.bm = p.bn = 256;
-        // A last round of fewer than half the CUs costs as much as a full one: its tile rows go to the small tiles instead
+        // A last round of fewer than half the CUs costs as much as a full one: its tile rows go to the small tiles instead.  One tile
+        // row that is wider than the whole rounds stays in one piece (200 x 82944 x 4096: 131 / 163 by 128 x 128 tiles)
         const long long over = t256 % kCUs;
-        const long long whole = t256 > kCUs && over > 0 && over <= kCUs / 2 ? (t256 - over) / nt : mt;
+        const long long whole = t256 > kCUs && over > 0 && over <= kCUs / 2 && t256 - over >= nt ? (t256 - over) / nt : mt;
         p.body = whole * 256 < M ? whole * 256 : M;
         return p;
     }
@@ -1195,6 +1196,16 @@ YFS_API int yfs_fp8_quantize_rows(const void* x, int dtype, int64_t ld, int64_t 
 YFS_API size_t yfs_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0 || M > kMost || N > kMost || K > kMost) return 0;
     return part_bytes(plan_tiles(M, N, (int)yfs_cdiv(K, 128), true), M, N);
+}
+
+YFS_API int yfs_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int out_dtype, int64_t* plan) {
+    YFS_REQUIRE(plan, YFS_ERR_INVALID_ARG, "yfs_fp8_gemm_plan: null pointer");
+    REQUIRE_SIZES("yfs_fp8_gemm_plan", M, N, K);
+    YFS_REQUIRE(known(out_dtype), YFS_ERR_UNSUPPORTED, "yfs_fp8_gemm_plan: unknown dtype %d", out_dtype);
+    const Plan p = plan_tiles(M, N, (int)yfs_cdiv(K, 128), out_dtype == YFS_F32);
+    const int64_t v[] = {p.bm, p.bn, p.splits, p.per_split, p.kind == 2 ? p.body : 0};
+    for (int i = 0; i < YFS_FP8_PLAN_LEN; ++i) plan[i] = v[i];
+    return YFS_OK;
 }
 
 YFS_API int yfs_fp8_gemm(const void* aq, const void* a_scale, const void* bq, const void* b_scale, int b_row_scales, const float* bias,
