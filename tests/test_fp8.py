@@ -690,3 +690,62 @@ def test_gradients_of_a_layer_with_more_than_65536_inputs(m):
     for n0 in range(0, n, 128):
         inner = inner + 2.0 ** -9 * dq[:, n0:n0 + 128].abs().amax(1, keepdim=True) * wq[n0:n0 + 128].abs().amax(0)
     assert bool(((dx.double() - ref).abs() <= 2.0 ** -8 * (ref.abs() + inner) + inner).all())
+
+
+def test_a_step_that_is_still_running_is_waited_for(monkeypatch):
+    """A weight whose overlapped optimiser step (FlatSGD.overlap_tail) may still be running is waited for before it is read:
+    by the quantiser, a frozen layer and the product, in that order."""
+    from yolo_from_scratch_amd import _lib as L
+    from yolo_from_scratch_amd import fp8_ops as f8
+    seen = []
+
+    class Owner:
+        def join(self):
+            seen.append("join")
+
+    class Ext:
+        def fp8_linear(self, *a):
+            seen.append("read")
+
+        fp8_linear_check = fp8_linear
+
+    def quantize(w, transposed):
+        seen.append("read")
+        return _cpu_weight(*w.shape) + (None, None)
+    lin = torch.nn.Linear(200, 40)
+    lin.weight._yfs_tail_owner, lin.weight._yfs_grad_sink = Owner(), torch.zeros(40, 200)
+    monkeypatch.setattr(f8, "_quantize_weight", quantize)
+    monkeypatch.setattr(L, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(L, "_binding", Ext())
+    monkeypatch.setattr(f8._SinkLinearFn, "apply", lambda *a: seen.append("read"))
+    f8.quantize_fp8(lin.weight)
+    assert seen == ["join", "read"]
+    f8.FrozenFp8Linear(lin)
+    assert seen == ["join", "read"] * 2
+    with torch.no_grad():
+        f8.fp8_linear(torch.zeros(3, 200), lin.weight)
+    assert seen == ["join", "read"] * 3
+    f8.fp8_linear(torch.zeros(3, 200), lin.weight)
+    assert seen == ["join", "read"] * 4 or seen == ["join", "read"] * 3 + ["join", "read", "read"]
+
+
+@pytest.mark.gpu
+def test_quantising_behind_an_overlapped_step():
+    """The step of a large layer runs on a side stream; what is quantised right behind it is the weight after the step."""
+    import yolo_from_scratch_amd as yfs
+    from yolo_from_scratch_amd import model as ym
+    from yolo_from_scratch_amd.train import FlatSGD
+    torch.manual_seed(6)
+    lin = ym.HipLinear(8192, 4096).to(DEV)
+    opt = FlatSGD(lin.parameters(), lr=0.5, momentum=0.9, overlap_tail=True)
+    x = torch.randn(64, 8192, device=DEV)
+    for _ in range(3):
+        opt.zero_grad()
+        lin(x).float().square().mean().backward()
+        opt.step(max_norm=None)
+        assert opt._tail is not None
+        q, frozen = yfs.quantize_fp8(lin.weight), yfs.FrozenFp8Linear(lin)
+        torch.cuda.synchronize()
+        want = yfs.quantize_fp8(lin.weight)
+        for got in (q.data, frozen.weight_data):
+            assert torch.equal(got.view(torch.uint8), want.data.view(torch.uint8))

@@ -77,6 +77,13 @@ def _check_weight(w):
         raise L.YfsError(f"quantize_fp8: expected a non-empty fp32, bf16 or fp16 matrix, got {w.dtype} {tuple(w.shape)}")
 
 
+def _settled(w):
+    """A parameter whose overlapped step (train.FlatSGD.overlap_tail) is still running on the side stream is waited for."""
+    owner = getattr(w, "_yfs_tail_owner", None)
+    if owner is not None:
+        owner.join()
+
+
 def _quantize_weight(w, transposed):
     """-> (data, scale) and, when asked, (data, scale) of the transpose: the same bytes, block by block."""
     w2, n, ld = _matrix(w.detach(), "quantize_fp8")
@@ -97,6 +104,7 @@ def quantize_fp8(w):
     """A weight matrix [n, k] (fp32, bf16 or fp16, rows with any stride) as ``Fp8Tensor``."""
     _check_weight(w)
     L.require_cuda(w)
+    _settled(w)
     q, s, _, _ = _quantize_weight(w, False)
     return Fp8Tensor(q, s, w.shape[1])
 
@@ -204,7 +212,10 @@ def fp8_linear(x, weight, bias=None):
     The backward pass multiplies in 8 bits too: dx = Q(dy) Q(weight), dW = Q(dy^T) Q(x^T)^T (summed in fp32, as the bias's
     gradient is); for it the transposed 8-bit weight and x are kept, not the 16-bit x."""
     ext = L._binding or L.binding()
-    if (getattr(weight, "_yfs_grad_sink", None) is None and getattr(bias, "_yfs_grad_sink", None) is None) or not torch.is_grad_enabled():
+    if getattr(weight, "_yfs_grad_sink", None) is None and getattr(bias, "_yfs_grad_sink", None) is None:
+        return ext.fp8_linear(x, weight, bias)
+    _settled(weight)
+    if not torch.is_grad_enabled():
         return ext.fp8_linear(x, weight, bias)
     ext.fp8_linear_check(x, weight, bias)
     return _SinkLinearFn.apply(x, weight, bias)
@@ -250,14 +261,12 @@ def freeze_fp8(model):
     puts the model into eval mode.  In place, all layers or (where one cannot be converted) none; a layer that stands in several
     places is converted once.  Returns the model."""
     from .model import HipLinear
-    from .train import bf16_shadow
     if isinstance(model, nn.Linear):
         raise L.YfsError("freeze_fp8: replaces the linear layers inside a module; for a layer alone: FrozenFp8Linear(layer)")
     places = [(m, name, c) for m in model.modules() for name, c in m._modules.items() if isinstance(c, nn.Linear)]
     frozen = {}
     for _, _, child in places:
         if child not in frozen:
-            bf16_shadow(child.weight)          # a step that is still running on the weight is waited for
             frozen[child] = FrozenFp8Linear(child, child.fused_act if isinstance(child, HipLinear) else None)
     for module, name, child in places:
         module._modules[name] = frozen[child]
