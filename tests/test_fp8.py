@@ -749,3 +749,17 @@ def test_quantising_behind_an_overlapped_step():
         want = yfs.quantize_fp8(lin.weight)
         for got in (q.data, frozen.weight_data):
             assert torch.equal(got.view(torch.uint8), want.data.view(torch.uint8))
+
+
+def test_packed_scales_must_be_aligned():
+    """The packed scales are fetched in dwords straight into LDS: q arrays and packed scales are 16-byte aligned, on both sides of
+    a product and in the quantiser."""
+    import yolo_from_scratch_amd as y
+    lib, p = y.lib(), 4096
+    gemm = lambda a, sa, b, sb, rows: lib.yfs_fp8_gemm(a, sa, b, sb, rows, None, p, 0, 8, 8, 8, 1.0, 1, None, 0, None)   # noqa: E731
+    for bad in range(4):
+        args = [p + 2 if i == bad else p for i in range(4)]
+        assert gemm(*args, 1) == -1
+    for off in (1, 8):
+        assert lib.yfs_fp8_quantize_rows(p, 0, 8, 8, 8, p, p + off, None, None, None, None) == -1
+        assert lib.yfs_fp8_quantize_rows(p, 0, 8, 8, 8, None, None, p, p + off, None, None) == -1

@@ -1187,6 +1187,8 @@ YFS_API int yfs_fp8_quantize_rows(const void* x, int dtype, int64_t ld, int64_t 
     YFS_REQUIRE(known(dtype), YFS_ERR_UNSUPPORTED, "yfs_fp8_quantize_rows: unknown dtype %d", dtype);
     REQUIRE_ALIGNED("yfs_fp8_quantize_rows", q);
     REQUIRE_ALIGNED("yfs_fp8_quantize_rows", qt);
+    REQUIRE_ALIGNED("yfs_fp8_quantize_rows", scale);
+    REQUIRE_ALIGNED("yfs_fp8_quantize_rows", scale_t);
     const QuantArgs g = {x, ld, M, K, (unsigned char*)q, (unsigned char*)scale, (unsigned char*)qt, (unsigned char*)scale_t, colsum,
                          groups64(M), groups64(K), 0, false};
     return quantize_rows(g, dtype, (hipStream_t)stream);
@@ -1221,6 +1223,7 @@ YFS_API int yfs_fp8_gemm(const void* aq, const void* a_scale, const void* bq, co
     REQUIRE_ALIGNED("yfs_fp8_gemm", aq);
     REQUIRE_ALIGNED("yfs_fp8_gemm", a_scale);
     REQUIRE_ALIGNED("yfs_fp8_gemm", bq);
+    if (b_row_scales) REQUIRE_ALIGNED("yfs_fp8_gemm", b_scale);
     const size_t need = yfs_fp8_gemm_workspace_bytes(M, N, K);
     YFS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), YFS_ERR_WORKSPACE, "yfs_fp8_gemm: workspace needs %zu bytes", need);
     GemmArgs g = {(const unsigned char*)aq, (const unsigned char*)a_scale, (const unsigned char*)bq, (const unsigned char*)b_scale, bias, out,
