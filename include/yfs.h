@@ -414,14 +414,15 @@ int yfs_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_t
                        void *workspace, size_t workspace_bytes, void *stream);
 
 /* LeakyReLU(slope) and dropout(p) whose mask is never stored: element e (row-major) is kept iff
- * (philox4x32_10(key = seed, counter = e / 4)[e % 4] >> 8) * 2^-24 >= p, the rule of yfs_fc_epilogue_fwd_bf16.
+ * (philox4x32_10(key = seed, counter = e / 4)[e % 4] >> 8) * 2^-24 >= p, the rule of yfs_fc_epilogue_fwd_bf16 (p rounded to
+ * fp32 for this comparison alone: the scale 1 / (1 - p) is that of p itself, rounded once).
  * fwd: y = keep ? leaky(x) / (1 - p) : 0.  bwd: dx = keep ? dy / (1 - p) * (y > 0 ? 1 : slope) : 0; y is read only when
  * slope != 1 (1: no activation).  n elements of `dtype`; 0 <= p <= 1, 0 <= slope <= 1.  seed_dev (may be NULL): a seed in
  * device memory that replaces `seed` and is read when the kernel runs, so that a captured graph draws a new mask at every
  * replay that changes it.  x == y and dy == dx are allowed. */
-int yfs_dropout_fwd(const void *x, void *y, int64_t n, float p, float slope, uint64_t seed, const int64_t *seed_dev, int dtype,
+int yfs_dropout_fwd(const void *x, void *y, int64_t n, double p, float slope, uint64_t seed, const int64_t *seed_dev, int dtype,
                     void *stream);
-int yfs_dropout_bwd(const void *dy, const void *y, void *dx, int64_t n, float p, float slope, uint64_t seed,
+int yfs_dropout_bwd(const void *dy, const void *y, void *dx, int64_t n, double p, float slope, uint64_t seed,
                     const int64_t *seed_dev, int dtype, void *stream);
 
 /* Measurement aid, no reference counterpart: enqueue a register-only bf16 MFMA loop (blocks x 4 waves x iters x

@@ -36,10 +36,10 @@ def keep_mask(seed, n, p):
 
 
 def dropout(x, p, seed, slope=1.0):
-    """-> y in 64 bits (p and slope as the fp32 numbers the kernels get)."""
+    """-> y in 64 bits.  p decides as an fp32 number, its scale is 1 / (1 - p); slope is the fp32 number the kernels get."""
     x = np.asarray(x, np.float64)
     keep = keep_mask(seed, x.size, p).reshape(x.shape)
-    scale = 0.0 if np.float32(p) >= 1 else 1.0 / (1.0 - float(np.float32(p)))
+    scale = 0.0 if np.float32(p) >= 1 else 1.0 / (1.0 - p)
     with np.errstate(invalid="ignore"):
         return np.where(keep, np.where(x > 0, x, x * float(np.float32(slope))) * scale, 0.0)
 
@@ -47,7 +47,7 @@ def dropout(x, p, seed, slope=1.0):
 def dropout_bwd(dy, y, p, seed, slope=1.0):
     dy = np.asarray(dy, np.float64)
     keep = keep_mask(seed, dy.size, p).reshape(dy.shape)
-    scale = 0.0 if np.float32(p) >= 1 else 1.0 / (1.0 - float(np.float32(p)))
+    scale = 0.0 if np.float32(p) >= 1 else 1.0 / (1.0 - p)
     with np.errstate(invalid="ignore"):
         return np.where(keep, dy * scale * (1.0 if slope == 1.0 else np.where(np.asarray(y, np.float64) > 0, 1.0, float(np.float32(slope)))), 0.0)
 

@@ -207,3 +207,24 @@ def test_any_whole_number_is_a_seed():
     want = yfs.dropout(x, 0.5, 7)
     assert torch.equal(yfs.dropout(x, 0.5, np.int64(7)), want) and torch.equal(yfs.dropout(x, 0.5, 7 + (1 << 64)), want)
     assert torch.equal(yfs.dropout(x, 0.5, -1), yfs.dropout(x, 0.5, (1 << 64) - 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("p", [0.1, 1 / 3, 0.9, 0.99, 0.999, 0.9999, 1 - 2.0 ** -20 + 2.0 ** -45])
+def test_scale_is_that_of_the_callers_p(p):
+    """Kept values are x / (1 - p) of the p that was given, which fp32 alone cannot hold near 1 (0.9999 in fp32 is off by 1.7e-4 of
+    1 - p): two roundings, of the scale and of the product, each half a step of 2^-23; three with a slope."""
+    import yolo_from_scratch_amd as yfs
+    g = torch.Generator().manual_seed(9)
+    x, dy = torch.randn(2, 1 << 22, generator=g).to(DEV)
+    for slope in (1.0, 0.1):
+        xg = x.clone().requires_grad_()
+        y = yfs.dropout(xg, p, 1234, slope)
+        dx, = torch.autograd.grad(y, xg, dy)
+        keep = y != 0
+        assert bool(keep.any())
+        neg = torch.where(x > 0, 1.0, float(np.float32(slope))).double()
+        for got, ref in ((y.detach(), x.double() * neg / (1 - p)), (dx, dy.double() * neg / (1 - p))):
+            err = (got.double() - ref).abs()[keep]
+            assert bool((err <= (2.001 if slope == 1.0 else 3.001) * 2.0 ** -24 * ref.abs()[keep]).all()), (slope, float((err / ref.abs()[keep]).max()))
+            assert bool((got[~keep] == 0).all())

@@ -38,7 +38,7 @@ def lib():
 
 # Entry points whose calls are short enough that ctypes' per-argument objects would show: their argument types are declared
 # once, so plain integers (data_ptr(), sizes, the raw stream) are passed as they are.  p pointer, l int64, z size_t, i int,
-# f float, u uint64.
+# f float, d double, u uint64.
 _SIGNATURES = {
     "yfs_layer_norm_fwd": "plppppp" "ll" "fi" "p",
     "yfs_layer_norm_bwd": "plpl" "ppp" "ppp" "ll" "i" "pz" "p",
@@ -57,11 +57,11 @@ _SIGNATURES = {
     "yfs_fp8_linear_fwd": "pil" "pil" "p" "pi" "lll" "i" "pz" "pz" "p",
     "yfs_fp8_linear_bwd": "pil" "pi" "pi" "pi" "lll" "i" "pz" "pz" "p",
     "yfs_fp8_colsum": "pllp" "i" "p",
-    "yfs_dropout_fwd": "ppl" "ff" "u" "p" "i" "p",
-    "yfs_dropout_bwd": "pppl" "ff" "u" "p" "i" "p",
+    "yfs_dropout_fwd": "ppl" "df" "u" "p" "i" "p",
+    "yfs_dropout_bwd": "pppl" "df" "u" "p" "i" "p",
 }
 _TYPES = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "z": ctypes.c_size_t, "i": ctypes.c_int, "f": ctypes.c_float,
-          "u": ctypes.c_uint64}
+          "d": ctypes.c_double, "u": ctypes.c_uint64}
 
 
 def _declare(handle):

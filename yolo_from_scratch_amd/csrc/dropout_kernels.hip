@@ -3,7 +3,8 @@
 //   element e of the tensor in row-major order is kept iff (philox4x32_10(key = seed, counter = e / 4)[e % 4] >> 8) 2^-24 >= p
 //   y = keep ? leaky(x) / (1 - p) : 0          dx = keep ? dy / (1 - p) (y > 0 ? 1 : slope) : 0
 // (the rule of yfs_fc_epilogue_fwd_bf16: the same seed and p keep the same elements there).
-// (r >> 8) 2^-24 >= p  <=>  r >= ceil(p 2^24) 2^8, a comparison of whole numbers prepared on the host.
+// (r >> 8) 2^-24 >= p  <=>  r >= ceil(p 2^24) 2^8, a comparison of whole numbers prepared on the host, with p rounded to fp32 (as
+// there).  The scale is that of p itself: near 1 its fp32 neighbour is off by much more of 1 - p than a rounding (0.9999: 1.7e-4).
 #include "yfs_common.h"
 #include "yfs_vec.h"
 #include <math.h>
@@ -79,31 +80,32 @@ int launch(DropArgs g, int dtype, hipStream_t s) {
     return YFS_OK;
 }
 
-int run(const char* name, bool bwd, const void* in, const void* y, void* out, int64_t n, float p, float slope, uint64_t seed,
+int run(const char* name, bool bwd, const void* in, const void* y, void* out, int64_t n, double p, float slope, uint64_t seed,
         const int64_t* seed_dev, int dtype, void* stream) {
     YFS_REQUIRE(in && out, YFS_ERR_INVALID_ARG, "%s: null pointer", name);
     YFS_REQUIRE(n > 0, YFS_ERR_INVALID_ARG, "%s: n must be positive (got %lld)", name, (long long)n);
-    YFS_REQUIRE(p >= 0.0f && p <= 1.0f, YFS_ERR_INVALID_ARG, "%s: p %g not in [0, 1]", name, p);
+    YFS_REQUIRE(p >= 0.0 && p <= 1.0, YFS_ERR_INVALID_ARG, "%s: p %g not in [0, 1]", name, p);
     YFS_REQUIRE(slope >= 0.0f && slope <= 1.0f, YFS_ERR_INVALID_ARG, "%s: slope %g not in [0, 1]", name, slope);
     YFS_REQUIRE(dtype == YFS_F32 || dtype == YFS_BF16 || dtype == YFS_F16, YFS_ERR_UNSUPPORTED, "%s: unknown dtype %d", name, dtype);
     const bool act = slope != 1.0f;
     YFS_REQUIRE(!bwd || !act || y, YFS_ERR_INVALID_ARG, "%s: the gradient of an activation needs y", name);
-    DropArgs g = {in, y, out, n, seed, (const long long*)seed_dev, 0u, 0u, p >= 1.0f, 0.0f, slope};
-    const double t = ceil((double)p * 16777216.0);
+    const float p32 = (float)p;
+    DropArgs g = {in, y, out, n, seed, (const long long*)seed_dev, 0u, 0u, p32 >= 1.0f, 0.0f, slope};
+    const double t = ceil((double)p32 * 16777216.0);
     g.thr = g.none ? 0xFFFFFFFFu : (unsigned)t << 8;
-    g.scale = g.none ? 0.0f : (float)(1.0 / (1.0 - (double)p));
+    g.scale = g.none ? 0.0f : (float)(1.0 / (1.0 - p));
     hipStream_t s = (hipStream_t)stream;
     if (bwd) return act ? launch<true, true>(g, dtype, s) : launch<true, false>(g, dtype, s);
     return act ? launch<false, true>(g, dtype, s) : launch<false, false>(g, dtype, s);
 }
 }  // namespace
 
-YFS_API int yfs_dropout_fwd(const void* x, void* y, int64_t n, float p, float slope, uint64_t seed, const int64_t* seed_dev,
+YFS_API int yfs_dropout_fwd(const void* x, void* y, int64_t n, double p, float slope, uint64_t seed, const int64_t* seed_dev,
                             int dtype, void* stream) {
     return run("yfs_dropout_fwd", false, x, nullptr, y, n, p, slope, seed, seed_dev, dtype, stream);
 }
 
-YFS_API int yfs_dropout_bwd(const void* dy, const void* y, void* dx, int64_t n, float p, float slope, uint64_t seed,
+YFS_API int yfs_dropout_bwd(const void* dy, const void* y, void* dx, int64_t n, double p, float slope, uint64_t seed,
                             const int64_t* seed_dev, int dtype, void* stream) {
     return run("yfs_dropout_bwd", true, dy, y, dx, n, p, slope, seed, seed_dev, dtype, stream);
 }

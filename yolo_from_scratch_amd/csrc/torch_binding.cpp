@@ -168,10 +168,10 @@ Tensor drop(bool backward, const Tensor& in, const Tensor& y, double p, double s
     const int64_t* where = seed_dev.defined() ? seed_dev.const_data_ptr<int64_t>() : nullptr;
     const int type = code(in.scalar_type());
     if (backward)
-        check(yfs.drop_bwd(ptr(in), ptr(y), out.mutable_data_ptr(), in.numel(), (float)p, (float)slope, (uint64_t)seed, where, type, stream_of(in)),
+        check(yfs.drop_bwd(ptr(in), ptr(y), out.mutable_data_ptr(), in.numel(), p, (float)slope, (uint64_t)seed, where, type, stream_of(in)),
               "yfs_dropout_bwd");
     else
-        check(yfs.drop_fwd(ptr(in), out.mutable_data_ptr(), in.numel(), (float)p, (float)slope, (uint64_t)seed, where, type, stream_of(in)),
+        check(yfs.drop_fwd(ptr(in), out.mutable_data_ptr(), in.numel(), p, (float)slope, (uint64_t)seed, where, type, stream_of(in)),
               "yfs_dropout_fwd");
     return out;
 }

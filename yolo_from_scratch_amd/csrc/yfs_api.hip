@@ -16,7 +16,7 @@ void yfs_set_error(const char* fmt, ...) {
     va_end(ap);
 }
 
-YFS_API int yfs_version(void) { return 300; }
+YFS_API int yfs_version(void) { return 301; }
 
 // ---- dispatch query: which conv kernel variant the calling thread's last conv entry point launched ------------------
 static thread_local char g_kernel[96] = {0};

@@ -13,8 +13,8 @@ from . import _lib as L
 
 def dropout(x, p, seed, slope=1.0):
     """LeakyReLU(slope) (1.0: none) and dropout of ``x`` (fp32, bf16 or fp16, any shape) as one kernel; element e of the
-    row-major tensor is kept iff (philox4x32_10(key=seed, counter=e // 4)[e % 4] >> 8) * 2**-24 >= p and then scaled by
-    1 / (1 - p).  Differentiable once.  ``seed``: an int (64 bits are used), or an int64 tensor of one element on x's GPU
+    row-major tensor is kept iff (philox4x32_10(key=seed, counter=e // 4)[e % 4] >> 8) * 2**-24 >= p (p rounded to
+    fp32 for this comparison) and then scaled by 1 / (1 - p).  Differentiable once.  ``seed``: an int (64 bits are used), or an int64 tensor of one element on x's GPU
     that the kernels read when they run (a captured graph then draws a new mask when the tensor is changed between replays;
     it must keep its value from the forward to the backward pass).  Nothing but the seed, and y where there is an
     activation, is kept for the backward pass.  0 <= p <= 1, 0 <= slope <= 1."""
