@@ -163,3 +163,31 @@ def test_feature_map_norm_behind_a_conv_block():
     y.float().square().sum().backward()
     for p in [x, *block.parameters(), *norm.parameters()]:
         assert p.grad is not None and torch.isfinite(p.grad).all()
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent of forward-mode differentiation is refused, not dropped, whichever argument carries it and whether or not the
+    tensor requires a gradient."""
+    import torch.autograd.forward_ad as fwd
+    import yolo_from_scratch_amd as yfs
+    from yolo_from_scratch_amd.fp8_ops import _pad
+    n, k = 40, 200
+    data = torch.zeros(n, _pad(k), dtype=torch.uint8).view(torch.float8_e4m3fn)
+    w8 = yfs.Fp8Tensor(data, torch.full((1, 2), 127, dtype=torch.uint8).view(torch.float8_e8m0fnu), k)
+    lin = yfs.Fp8Linear(k, n)
+    lin.weight._yfs_grad_sink = torch.zeros(n, k)
+    x, w, wk, b = torch.zeros(3, k), torch.zeros(n, k), torch.ones(k), torch.zeros(n)
+    with fwd.dual_level():
+        for grad in (False, True):
+            dual = lambda t: fwd.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))   # noqa: E731
+            for call in (lambda: yfs.layer_norm(dual(x)), lambda: yfs.layer_norm(x, dual(wk)), lambda: yfs.layer_norm(x, wk, dual(wk)),
+                         lambda: yfs.dropout(dual(x), 0.5, 1), lambda: yfs.fp8_linear(dual(x), w), lambda: yfs.fp8_linear(x, dual(w)),
+                         lambda: yfs.fp8_linear(x, w, dual(b)), lambda: yfs.fp8_linear(dual(x), lin.weight, lin.bias),
+                         lambda: yfs.fp8_matmul(dual(x), w8), lambda: yfs.fp8_matmul(x, w8, dual(b)), lambda: yfs.quantize_fp8(dual(w))):
+                with pytest.raises(yfs.YfsError, match="forward-mode"):
+                    call()
+                with torch.no_grad(), pytest.raises(yfs.YfsError, match="forward-mode"):
+                    call()
+        for call in (lambda: yfs.layer_norm(x), lambda: yfs.dropout(x, 0.5, 1), lambda: yfs.fp8_linear(x, w), lambda: yfs.fp8_matmul(x, w8)):
+            with pytest.raises(yfs.YfsError, match="CPU tensor"):      # (no tangent: the next refusal)
+                call()

@@ -49,8 +49,15 @@ void check(int status, const char* what) {
 int code(at::ScalarType t) {
     return t == at::kFloat ? YFS_F32 : (t == at::kBFloat16 ? YFS_BF16 : (t == at::kHalf ? YFS_F16 : -1));
 }
-// all on one GPU
+// a tangent of forward-mode differentiation would be dropped without a word where no gradient is required
+void no_tangent(const char* what, std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t && t->defined() && t->_fw_grad(/*level=*/0).defined())
+            fail(c10::str(what, ": forward-mode derivatives are not implemented, and an argument carries a tangent"));
+}
+// all on one GPU, without tangents
 void on_one_gpu(const char* what, std::initializer_list<const Tensor*> ts) {
+    no_tangent(what, ts);
     const Tensor* first = nullptr;
     for (const Tensor* t : ts) {
         if (!t || !t->defined()) continue;

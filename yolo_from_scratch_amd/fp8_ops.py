@@ -12,6 +12,7 @@ x / s is rounded to nearest, ties to even.  NaN and infinities become NaN, witho
 """
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -103,6 +104,8 @@ def _quantize_weight(w, transposed):
 def quantize_fp8(w):
     """A weight matrix [n, k] (fp32, bf16 or fp16, rows with any stride) as ``Fp8Tensor``."""
     _check_weight(w)
+    if forward_ad.unpack_dual(w).tangent is not None:
+        raise L.YfsError("quantize_fp8: forward-mode derivatives are not implemented, and w carries a tangent")
     L.require_cuda(w)
     _settled(w)
     q, s, _, _ = _quantize_weight(w, False)
