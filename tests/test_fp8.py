@@ -763,3 +763,22 @@ def test_packed_scales_must_be_aligned():
     for off in (1, 8):
         assert lib.yfs_fp8_quantize_rows(p, 0, 8, 8, 8, p, p + off, None, None, None, None) == -1
         assert lib.yfs_fp8_quantize_rows(p, 0, 8, 8, 8, None, None, p, p + off, None, None) == -1
+
+
+@pytest.mark.gpu
+def test_backward_through_a_stored_weight_is_refused():
+    """fp8_matmul has no gradient: a backward pass that reaches it says so, instead of leaving out what lies in front of it."""
+    import yolo_from_scratch_amd as yfs
+    wq = yfs.quantize_fp8(_matrix(40, 200, 71))
+    frozen = yfs.FrozenFp8Linear(torch.nn.Linear(200, 40).to(DEV))
+    front = _matrix(20, 200, 72).requires_grad_()
+    bias = torch.randn(40, device=DEV, requires_grad=True)
+    h = (2 * front).bfloat16()
+    for y in (yfs.fp8_matmul(h, wq), frozen(h), yfs.fp8_matmul(h.detach(), wq, bias), yfs.fp8_matmul(front, wq), yfs.fp8_matmul(h[:0], wq)):
+        loss = y.float().sum() + front.sum() + bias.sum()
+        with pytest.raises(RuntimeError, match="fp8_matmul.*not differentiable"):
+            loss.backward()
+    with torch.no_grad():
+        assert yfs.fp8_matmul(h, wq).grad_fn is None
+    assert yfs.fp8_matmul(h.detach(), wq, bias.detach()).grad_fn is None and not frozen(h.detach()).requires_grad
+    assert torch.equal(yfs.fp8_matmul(h, wq), yfs.fp8_matmul(h.detach(), wq))

@@ -5,6 +5,8 @@
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -225,8 +227,8 @@ Tensor dropout(const Tensor& x, double p, const py::object& seed, double slope) 
 }
 
 // ---- served 8-bit product --------------------------------------------------------------------------------------------
-Tensor fp8_matmul(const Tensor& x, const Tensor& data, const Tensor& scale, int64_t k, const OptTensor& bias, std::optional<double> slope_,
-                  const std::optional<at::ScalarType>& out_dtype) {
+Tensor matmul_forward(const Tensor& x, const Tensor& data, const Tensor& scale, int64_t k, const Tensor& b, std::optional<double> slope_,
+                      const std::optional<at::ScalarType>& out_dtype) {
     if (x.dim() == 0 || x.size(-1) != k) fail(c10::str("fp8_matmul: x [..., ", k, "] expected, got ", x.sizes()));
     if (code(x.scalar_type()) < 0) fail(c10::str("fp8_matmul: x must be fp32, bf16 or fp16, got ", x.scalar_type()));
     const at::ScalarType out = out_dtype.value_or(x.scalar_type());
@@ -234,7 +236,6 @@ Tensor fp8_matmul(const Tensor& x, const Tensor& data, const Tensor& scale, int6
     const double slope = slope_.value_or(1.0);
     if (!(slope >= 0.0 && slope <= 1.0)) fail(c10::str("fp8_matmul: slope must lie in [0, 1], got ", slope));
     const int64_t n = data.size(0);
-    const Tensor b = get(bias);
     if (b.defined() && (b.dim() != 1 || b.size(0) != n || !b.is_floating_point()))
         fail(c10::str("fp8_matmul: bias must be floating point [", n, "], got ", str(b)));
     on_one_gpu("fp8_matmul", {&x, &data, &scale, &b});
@@ -251,6 +252,17 @@ Tensor fp8_matmul(const Tensor& x, const Tensor& data, const Tensor& scale, int6
     check(yfs.matmul(ptr(r.t), code(x.scalar_type()), r.stride, ptr(data), ptr(scale), f32(bf), y.mutable_data_ptr(), code(out), r.rows, n, k,
                      (float)slope, bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(x)),
           "yfs_fp8_matmul");
+    return y;
+}
+Tensor fp8_matmul(const Tensor& x, const Tensor& data, const Tensor& scale, int64_t k, const OptTensor& bias, std::optional<double> slope,
+                  const std::optional<at::ScalarType>& out_dtype) {
+    const Tensor b = get(bias);
+    Tensor y = matmul_forward(x, data, scale, k, b, slope, out_dtype);
+    // A backward pass that comes here is refused.  The node has no edges: with them a result that is kept would keep the leaves'
+    // graph alive, beside which no backward pass of theirs can be captured.
+    if (at::GradMode::is_enabled() && (x.requires_grad() || (b.defined() && b.requires_grad())))
+        torch::autograd::set_history(y, std::make_shared<torch::autograd::Error>(
+            "fp8_matmul: not differentiable (fp8_linear is; without gradients: torch.no_grad() or x.detach())"));
     return y;
 }
 
