@@ -782,3 +782,23 @@ def test_backward_through_a_stored_weight_is_refused():
         assert yfs.fp8_matmul(h, wq).grad_fn is None
     assert yfs.fp8_matmul(h.detach(), wq, bias.detach()).grad_fn is None and not frozen(h.detach()).requires_grad
     assert torch.equal(yfs.fp8_matmul(h, wq), yfs.fp8_matmul(h.detach(), wq))
+
+
+@pytest.mark.gpu
+def test_two_backward_passes_over_a_retained_graph():
+    """A layer bound to an optimiser's arena takes several backward passes over one graph, as any other does: twice the gradient,
+    which is exact, and the same dx."""
+    import yolo_from_scratch_amd as yfs
+    from yolo_from_scratch_amd.train import FlatSGD
+    torch.manual_seed(11)
+    for bias in (True, False):
+        lin = yfs.Fp8Linear(300, 140, bias=bias).to(DEV)
+        opt = FlatSGD(lin.parameters(), lr=0.01, momentum=0.9)
+        x = torch.randn(90, 300, device=DEV, requires_grad=True)
+        opt.zero_grad()
+        loss = lin(x).float().square().sum()
+        loss.backward(retain_graph=True)
+        once = [p.grad.clone() for p in (x, *lin.parameters())]
+        loss.backward()
+        for p, g in zip((x, *lin.parameters()), once):
+            assert torch.equal(p.grad, g + g)

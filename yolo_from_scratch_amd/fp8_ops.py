@@ -207,7 +207,6 @@ class _SinkLinearFn(torch.autograd.Function):
                 if not direct:
                     sink.add_(out) if accumulate else sink.copy_(out)
             results.append(write_grad(param, put) if out is not None else None)
-        ctx.wb = None
         return dx, results[0], results[1]
 
 
