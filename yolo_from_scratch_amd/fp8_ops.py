@@ -168,10 +168,12 @@ class _SinkLinearFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        from .train import write_grad
+        from .train import settle_deferred, write_grad
         shape, dtype, m, n, k, needs = ctx.meta
         weight, bias = ctx.wb
         need_x, need_w, need_b = ctx.needs_input_grad
+        if need_w:
+            settle_deferred(weight)      # a layer in 16 bits that shares it may have left its gradient as factors
         if m == 0:
             return (dy.new_empty(shape) if need_x else None, torch.zeros_like(weight) if need_w else None,
                     torch.zeros_like(bias) if need_b else None)

@@ -444,7 +444,7 @@ class _LinearFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        from .train import write_grad
+        from .train import settle_deferred, write_grad
         (x16,) = ctx.saved_tensors
         w16 = ctx.w16
         weight, bias = ctx.wb
@@ -467,17 +467,10 @@ class _LinearFn(torch.autograd.Function):
         dx = torch.mm(dy16, w16).to(ctx.in_dtype) if ctx.needs_input_grad[0] else None
 
         sink_w = getattr(weight, "_yfs_grad_sink", None)
-        pending = getattr(weight, "_yfs_factors", None)
         comm = getattr(weight, "_yfs_comm", None)
         multi = comm is not None and getattr(comm, "active", getattr(comm, "world", 1) > 1)
-        if pending is not None and sink_w is not None:
-            # a second backward before the step: the deferred factors become an ordinary gradient first
-            if multi:
-                raise L.YfsError("several backward passes per step are not supported together with the deferred Linear "
-                                 "gradient under data parallelism (set YFS_DEFER_FC=0)")
-            torch.mm(pending[1].t(), pending[0], out_dtype=torch.float32, out=sink_w)
-            weight._yfs_factors = None
-        elif getattr(weight, "_yfs_defer", False) and sink_w is not None and weight._yfs_grad_fresh:
+        settle_deferred(weight)          # (then the gradient is no longer fresh: this one is added to it)
+        if getattr(weight, "_yfs_defer", False) and sink_w is not None and weight._yfs_grad_fresh:
             # FlatSGD takes this layer's step from the factors of its gradient (train.FlatSGD._step_with_deferred);
             # with several ranks the factors of all ranks are gathered and the mean gradient is 1/world of their product
             if multi:

@@ -301,6 +301,19 @@ def bf16_shadow(param):
     return sh
 
 
+def settle_deferred(param):
+    """A second backward before the step: the deferred factors of ``param``'s gradient become an ordinary gradient first."""
+    pending = getattr(param, "_yfs_factors", None)
+    if pending is None:
+        return
+    comm = getattr(param, "_yfs_comm", None)
+    if comm is not None and getattr(comm, "active", getattr(comm, "world", 1) > 1):
+        raise L.YfsError("several backward passes per step are not supported together with the deferred Linear "
+                         "gradient under data parallelism (set YFS_DEFER_FC=0)")
+    torch.mm(pending[1].t(), pending[0], out_dtype=torch.float32, out=param._yfs_grad_sink)
+    param._yfs_factors = None
+
+
 def write_grad(param, value_fn):
     """Used by this package's autograd nodes: if ``param`` has a gradient sink, let ``value_fn(sink, accumulate)``
     write into it and return None (autograd then has nothing to accumulate); otherwise return the gradient."""
