@@ -361,7 +361,7 @@ typedef enum { YFS_F32 = 0, YFS_BF16 = 1, YFS_F16 = 2 } yfs_dtype;
  * aligned.  x and w: `dtype` elements, ld elements from row to row, any alignment.
  * yfs_fp8_quantize_weight: qt / scale_t (both or neither NULL) = the transpose, [K, pad(N)] and [ceil(K/128), ceil(N/128)].
  * yfs_fp8_quantize_rows: q / scale = x by rows; qt / scale_t = x^T by rows (blocks of 128 rows of x), [K, pad(M)]; either pair
- *   may be NULL.  colsum (may be NULL) [ceil(M/128), K]: sums of x over each 128 rows; yfs_fp8_colsum adds them up in order. */
+ *   may be NULL.  colsum (may be NULL) [ceil(M/128), K]: sums of x over each 128 rows; yfs_fp8_colsum adds them up in a fixed order. */
 int yfs_fp8_quantize_weight(const void *w, int dtype, int64_t ld, int64_t N, int64_t K, void *q, void *scale, void *qt,
                             void *scale_t, void *stream);
 size_t yfs_fp8_packed_scale_bytes(int64_t rows, int64_t cols);

@@ -827,3 +827,21 @@ def test_weight_shared_with_a_layer_whose_gradient_is_deferred(deferred_first):
     assert getattr(lin.weight, "_yfs_factors", None) is None
     for got, a, b in ((lin.weight.grad, ga, gb), (lin.bias.grad, gab, gbb)):     # products with sums in fp32, one more rounding
         assert bool(((got - (a + b)).abs() <= 2.0 ** -22 * (a.abs() + b.abs()) + 2.0 ** -24 * 70 * 20).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [129, 4096, 4097, 200704, 1000003])
+def test_bias_gradient_over_many_rows(m):
+    """The 128-row sums are joined by 32 chains and these in turn, so that what a column loses grows with a 32nd of the rows: 7
+    roundings in a tile of 128 rows, one for each 32nd tile, 31 behind them.  Equal values lose most, all in one direction."""
+    import yolo_from_scratch_amd as yfs
+    c = torch.tensor([1.0, 1.1, 1 / 3, -0.7, 1.0000001, 123.456, -1e-3, 3.3, 0.6, 1.9], device=DEV)
+    dy = c.expand(m, 10).contiguous()
+    dy[:, 9] = torch.randn(m, device=DEV, generator=torch.Generator(DEV).manual_seed(m))
+    x = torch.ones(m, 4, device=DEV)
+    w, b = torch.ones(10, 4, device=DEV, requires_grad=True), torch.zeros(10, device=DEV, requires_grad=True)
+    _, db = torch.autograd.grad(yfs.fp8_linear(x, w, b), (w, b), dy)
+    chain = 7 + -(-(-(-m // 128)) // 32) + 31
+    err = (db.double() - dy.double().sum(0)).abs()
+    assert bool((err <= chain * 2.0 ** -24 * dy.double().abs().sum(0)).all()), (err / dy.double().abs().sum(0) * 2 ** 24).tolist()
+    assert torch.equal(torch.autograd.grad(yfs.fp8_linear(x, w, b), (w, b), dy)[1], db)

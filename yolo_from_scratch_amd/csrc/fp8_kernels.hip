@@ -252,14 +252,25 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(QuantArgs g) {
     }
 }
 
-// sums over quant_rows_kernel's colsum, in the order of the rows
-__global__ void __launch_bounds__(256) colsum_kernel(const float* __restrict__ part, long long tiles, long long K,
-                                                     float* __restrict__ out, int accumulate) {
-    const long long k = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (k >= K) return;
+// Sums over quant_rows_kernel's colsum: 32 columns x 32 slices of the tiles (8 where there are at most 64 tiles: 5 x 50176 3.1 us
+// against 3.8), joined in slice order.  A chain of roundings is tiles / 32 + 31 long and its loads are on their way together (1568 x
+// 4096: 4 us; as one chain over the tiles 161 us, and equal values lost 240 half steps of their sum).
+__global__ void __launch_bounds__(1024) colsum_kernel(const float* __restrict__ part, long long tiles, long long K,
+                                                      float* __restrict__ out, int accumulate) {
+    __shared__ float red[32][33];
+    const int ct = threadIdx.x & 31, slice = threadIdx.x >> 5, slices = (int)blockDim.x >> 5;
+    const long long k = (long long)blockIdx.x * 32 + ct;
     float s = 0.0f;
-    for (long long t = 0; t < tiles; ++t) s += part[t * K + k];
-    out[k] = accumulate ? out[k] + s : s;
+    if (k < K) {
+#pragma unroll 4
+        for (long long t = slice; t < tiles; t += slices) s += part[t * K + k];
+    }
+    red[slice][ct] = s;
+    __syncthreads();
+    if (slice == 0 && k < K) {
+        for (int q = 1; q < slices; ++q) s += red[q][ct];
+        out[k] = accumulate ? out[k] + s : s;
+    }
 }
 
 template <bool COLQ>
@@ -1279,8 +1290,9 @@ YFS_API int yfs_fp8_matmul(const void* x, int x_dtype, int64_t ld, const void* w
 }
 
 YFS_API int yfs_fp8_colsum(const float* part, int64_t tiles, int64_t K, float* out, int accumulate, void* stream) {
-    YFS_REQUIRE(part && out && tiles > 0 && K > 0, YFS_ERR_INVALID_ARG, "yfs_fp8_colsum: null pointer or size <= 0");
-    colsum_kernel<<<dim3((unsigned)yfs_cdiv(K, 256)), 256, 0, (hipStream_t)stream>>>(part, tiles, K, out, accumulate);
+    YFS_REQUIRE(part && out, YFS_ERR_INVALID_ARG, "yfs_fp8_colsum: null pointer");
+    REQUIRE_SIZES("yfs_fp8_colsum", tiles, 1, K);
+    colsum_kernel<<<dim3((unsigned)yfs_cdiv(K, 32)), tiles <= 64 ? 256 : 1024, 0, (hipStream_t)stream>>>(part, tiles, K, out, accumulate);
     YFS_CHECK_LAUNCH("colsum_kernel");
     return YFS_OK;
 }
