@@ -228,3 +228,50 @@ def test_scale_is_that_of_the_callers_p(p):
             err = (got.double() - ref).abs()[keep]
             assert bool((err <= (2.001 if slope == 1.0 else 3.001) * 2.0 ** -24 * ref.abs()[keep]).all()), (slope, float((err / ref.abs()[keep]).max()))
             assert bool((got[~keep] == 0).all())
+
+
+@pytest.mark.gpu
+def test_module_draws_a_new_mask_at_every_replay():
+    """A captured HipDropout draws its seed on the GPU, from the generator whose state a graph advances: other elements at every
+    replay, the same ones forward and backward, the same series from the same state; eager calls between replays."""
+    import yolo_from_scratch_amd as yfs
+    m = yfs.HipDropout(0.3, slope=0.1)
+    x = torch.randn(257, 1000, device=DEV)
+    dy = torch.randn(257, 1000, device=DEV)
+    xg = x.clone().requires_grad_()
+
+    def step():
+        y = m(xg)
+        return y.detach(), torch.autograd.grad(y, xg, dy)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            y, dx = step()
+    torch.cuda.current_stream().wait_stream(side)
+    scale = torch.where(x > 0, 1.0, float(np.float32(0.1))).double() / 0.7
+    series = []
+    for run in range(2):
+        torch.cuda.manual_seed(77)
+        seen = []
+        for _ in range(4):
+            y.fill_(9), dx.fill_(9)
+            graph.replay()
+            torch.cuda.synchronize()
+            keep = y != 0
+            assert abs(float(keep.float().mean()) - 0.7) < 0.01 and torch.equal(dx != 0, keep & (dy != 0))
+            for got, ref in ((y, x.double() * scale), (dx, dy.double() * scale)):
+                assert bool(((got.double() - ref).abs()[keep] <= 3.001 * 2.0 ** -24 * ref.abs()[keep]).all())
+            seen.append(keep)
+            m(x), yfs.dropout(x, 0.5, 3)
+        assert not any(torch.equal(a, b) for i, a in enumerate(seen) for b in seen[:i])
+        series.append(torch.stack(seen))
+    assert torch.equal(*series)
+
+
+def test_module_refuses_a_cpu_tensor():
+    import yolo_from_scratch_amd as yfs
+    with pytest.raises(yfs.YfsError, match="CPU tensor"):
+        yfs.HipDropout(0.3)(torch.zeros(4, 8))

@@ -23,8 +23,8 @@ def dropout(x, p, seed, slope=1.0):
 
 class HipDropout(nn.Module):
     """nn.LeakyReLU(slope) (1.0: none) and nn.Dropout(p) as one kernel without a stored mask.  In training each call draws
-    its seed from torch's CPU generator, as ``HipLinear`` does (reproducible under torch.manual_seed); in eval mode the
-    activation alone is applied."""
+    its seed from torch's CPU generator, as ``HipLinear`` does (reproducible under torch.manual_seed); while a graph is captured,
+    from the GPU's, so that every replay draws a mask of its own.  In eval mode the activation alone is applied."""
 
     def __init__(self, p=0.5, slope=1.0):
         super().__init__()
@@ -36,7 +36,12 @@ class HipDropout(nn.Module):
         p = self.p if self.training else 0.0
         if p == 0.0 and self.slope == 1.0:
             return x
-        seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if p > 0 else 0
+        if p == 0.0:
+            seed = 0
+        elif x.is_cuda and torch.cuda.is_current_stream_capturing():
+            seed = torch.randint(0, 2 ** 62, (1,), device=x.device)
+        else:
+            seed = int(torch.randint(0, 2 ** 62, (1,)).item())
         return dropout(x, p, seed, self.slope)
 
     def extra_repr(self):
