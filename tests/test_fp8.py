@@ -845,3 +845,31 @@ def test_bias_gradient_over_many_rows(m):
     err = (db.double() - dy.double().sum(0)).abs()
     assert bool((err <= chain * 2.0 ** -24 * dy.double().abs().sum(0)).all()), (err / dy.double().abs().sum(0) * 2 ** 24).tolist()
     assert torch.equal(torch.autograd.grad(yfs.fp8_linear(x, w, b), (w, b), dy)[1], db)
+
+
+def test_tolerance_covers_every_plan():
+    """The 96 + K / 32 half steps that the products are held to, from the plans themselves: 32 products in one matrix instruction,
+    four instructions for each block of 128 of a part, and one addition for each part (98 of them at 64 x 128 x 50176).  A layer
+    that trains with up to 64 rows has at most 128 parts of two blocks or more: 4 K / (128 parts) + parts <= K / 32 there too."""
+    import random
+    rng = random.Random(8)
+    most = 0
+    for _ in range(20000):
+        m, n, k = [max(1, int(2 ** rng.uniform(0, top))) for top in (15, 17, 17)]
+        _, _, parts, per, _ = _plan(m, n, k, torch.float32)
+        assert parts == 1 or per >= 4 and parts <= k / 512 + 1, (m, n, k)
+        assert 32 + 4 * per + parts - 1 <= 96 + k / 32, (m, n, k)
+        most = max(most, parts)
+    assert most > 64
+
+
+@pytest.mark.gpu
+def test_second_derivative_in_an_optimisers_arena_is_refused():
+    import yolo_from_scratch_amd as yfs
+    from yolo_from_scratch_amd.train import FlatSGD
+    lin = yfs.Fp8Linear(64, 8).to(DEV)
+    FlatSGD(lin.parameters(), lr=0.1)
+    x = torch.randn(4, 64, device=DEV, requires_grad=True)
+    g, = torch.autograd.grad(lin(x).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()

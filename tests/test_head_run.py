@@ -191,3 +191,61 @@ def test_forward_mode_derivatives_are_refused():
         for call in (lambda: yfs.layer_norm(x), lambda: yfs.dropout(x, 0.5, 1), lambda: yfs.fp8_linear(x, w), lambda: yfs.fp8_matmul(x, w8)):
             with pytest.raises(yfs.YfsError, match="CPU tensor"):      # (no tangent: the next refusal)
                 call()
+
+
+@pytest.mark.gpu
+def test_create_graph_is_refused_by_the_backward_pass_itself():
+    import yolo_from_scratch_amd as yfs
+    x = torch.randn(4, 32, device=DEV, requires_grad=True)
+    w = torch.ones(8, 32, device=DEV, requires_grad=True)
+    for f in (lambda: yfs.layer_norm(x), lambda: yfs.dropout(x, 0.5, 1), lambda: yfs.fp8_linear(x, w)):
+        y = f().sum()
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad(y, x, create_graph=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("norm", [False, True])
+def test_frozen_form_of_a_head_trained_in_16_bits(norm):
+    """Every stage of the frozen head is the 8-bit product of its quantised weight, with its bias and its activation, and fc.1 stays
+    within the two roundings to e4m3 of its 16-bit form: half a step of 2^-3 each and their product, 2^-10 of the largest value
+    of a block (x: of the row's, w: of the 128 x 128 block's) for what lies in the subnormal range, then the 16-bit sums' own error."""
+    import yolo_from_scratch_amd as yfs
+    from yolo_from_scratch_amd import model as ym
+    torch.manual_seed(4)
+    net = ym.YoloRegressorModel(head_out=30, image_size=64, head_norm=norm).to(DEV).eval()
+    with torch.no_grad():
+        for i in (1, 4):
+            net.fc[i].bias.normal_()
+        if norm:
+            net.fc[2].weight.uniform_(0.5, 1.5), net.fc[2].bias.normal_()
+        x = torch.rand(6, 3, 64, 64, device=DEV)
+        flat = net.feat(x).flatten(1)
+        w1, b1, w4, b4 = [t.detach().clone() for i in (1, 4) for t in (net.fc[i].weight, net.fc[i].bias)]
+        plain, hidden16 = net(x), net.fc[1](flat).float()
+        q1, q4 = yfs.quantize_fp8(w1), yfs.quantize_fp8(w4)
+        served = yfs.freeze_fp8(net)
+        assert torch.equal(served.feat(x).flatten(1), flat)
+        slope = None if norm else ym.SLOPE
+        h = yfs.fp8_matmul(flat, q1, b1, slope, torch.bfloat16)
+        assert torch.equal(served.fc[1](flat), h)
+        if norm:
+            a = yfs.dropout(yfs.layer_norm(h, net.fc[2].weight, net.fc[2].bias), 0.0, 0, ym.SLOPE)
+        else:
+            a = h
+        want = yfs.fp8_matmul(a, q4, b4, None, torch.bfloat16).float()
+        assert torch.equal(served(x), want) and not torch.equal(want, plain)
+
+    f, w = _np(flat), _np(w1)
+    k = f.shape[1]
+    top = lambda t: np.abs(t).reshape(t.shape[0], k // 128, 128).max(2)   # noqa: E731
+    fe = np.abs(f) * 2.0 ** -4 + np.repeat(top(f), 128, 1) * 2.0 ** -17      # half a subnormal step is 2^-10 s, and s < max / 224
+    wt = top(w).reshape(-1, 128, k // 128).max(1)                           # of a 128 x 128 block
+    we = np.abs(w) * 2.0 ** -4 + np.repeat(np.repeat(wt, 128, 0), 128, 1) * 2.0 ** -17
+    bound = np.abs(f) @ we.T + fe @ np.abs(w).T + fe @ we.T
+    bound += np.abs(f) @ np.abs(w).T * 2.0 ** -8 + 2.0 ** -7 * np.abs(_np(hidden16))     # bf16 weights and results, the 8-bit sums
+    ref = f @ w.T + _np(b1)
+    if slope is not None:
+        ref = np.where(ref > 0, ref, slope * ref)
+    for got in (_np(h), _np(hidden16)):
+        assert (np.abs(got - ref) <= bound + 2.0 ** -7 * np.abs(ref) + 1e-6).all()
