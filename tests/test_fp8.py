@@ -873,3 +873,32 @@ def test_second_derivative_in_an_optimisers_arena_is_refused():
     g, = torch.autograd.grad(lin(x).float().square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("axis", [0, 1, 2])
+def test_longest_axes(axis):
+    """The largest size along each axis, 2^23 - 256: forward, all three gradients, and the served form.  Operands are small whole
+    numbers, which 8 bits hold, so that a sum is exact as far as it stays below 2^24.  y of the longest reduction reaches 4 * (2^23 - 256),
+    between 2^24 and 2^25: its parts of 256 blocks are below 2^18 and exact, and each of the 256 additions that join them, and the
+    bias's, rounds by half a step of 2 at most: 257 half steps, 257 * 2^-24 of the sum at most."""
+    import yolo_from_scratch_amd as yfs
+    big = (1 << 23) - 256
+    m, n, k = [big if i == axis else 1 for i in range(3)]
+    i = lambda c, mod: (torch.arange(c, device=DEV) % mod - mod // 2).float()   # noqa: E731
+    x = (i(m, 3)[:, None] + i(k, 5)[None]).bfloat16().requires_grad_()
+    w = (i(n, 5)[:, None] * (i(k, 3)[None] + 2)).requires_grad_()
+    b = i(n, 7).requires_grad_()
+    dy = (i(m, 5)[:, None] + i(n, 3)[None]).bfloat16()
+    xd, wd, dd = x.detach().double(), w.detach().double(), dy.double()
+    y = yfs.fp8_linear(x, w, b)
+    ref = xd @ wd.t() + b.detach().double()
+    close = lambda got, ref: bool(((got.double() - ref).abs() <= 2.0 ** -8 * ref.abs()).all())   # noqa: E731
+    assert close(y.detach(), ref)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert close(dx, dd @ wd) and torch.equal(dw.double(), dd.t() @ xd) and torch.equal(db.double(), dd.sum(0))
+    with torch.no_grad():
+        wq = yfs.quantize_fp8(w)
+        assert torch.equal(wq.dequantize(), w)
+        err = (yfs.fp8_matmul(x, wq, b, out_dtype=torch.float32).double() - ref).abs()
+        assert bool((err <= (257 * 2.0 ** -24 * ref.abs() if axis == 2 else 0 * ref)).all()) and close(yfs.fp8_matmul(x, wq, b), ref)
