@@ -284,8 +284,9 @@ __device__ __forceinline__ void column_sums(const BwdArgs& g, int block, float* 
 // dx by rows as in the forward pass.  ACC: the thread that holds a column of dx sums its dw and db too, over the rows that its
 // workgroup meets: x and dy are read once for all three (200704 x 256 bf16: 55 us, 5.6 TB/s; 53 + 114 as two kernels).  That needs
 // many rows per workgroup, or the partial sums outgrow them; for few rows the column sums are other workgroups of the same launch.
+// Four waves a SIMD at least, as the plan counts on: odd bf16 rows took 130 registers and then 188 us where 50000 x 1470 takes 130.
 template <typename T, int NV, bool BLOCK, bool ACC, bool ODD>
-__global__ void __launch_bounds__(BLOCK ? 512 : 256) ln_bwd_kernel(BwdArgs g) {
+__global__ void __launch_bounds__(BLOCK ? 512 : 256, 4) ln_bwd_kernel(BwdArgs g) {
     constexpr int VE = 16 / sizeof(T);
     __shared__ float2 red[32];
     extern __shared__ float sums[];
