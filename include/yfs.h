@@ -370,8 +370,8 @@ int yfs_fp8_quantize_rows(const void *x, int dtype, int64_t ld, int64_t M, int64
 int yfs_fp8_colsum(const float *part, int64_t tiles, int64_t K, float *out, int accumulate, void *stream);
 /* out [M, N] = leaky(a b^T + bias): a [M, K] with packed row scales, b [N, K] with packed row scales (b_row_scales != 0; fp32
  * outputs only) or 128 x 128 scales.  bias [N] fp32 or NULL; slope 1 = no activation.  out_dtype fp32: full fp32 sums, accumulate != 0 adds to
- * what is there (before the activation); bf16 / fp16: the e4m3 matrix instructions, whose sums over one block keep about 16
- * bits behind the largest product. */
+ * what is there (before the activation); bf16 / fp16: the e4m3 matrix instructions, whose sums over one block keep 16 bits
+ * behind the largest product: off by 2^-9 of it for each block at most. */
 size_t yfs_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int yfs_fp8_gemm(const void *aq, const void *a_scale, const void *bq, const void *b_scale, int b_row_scales, const float *bias,
                  void *out, int out_dtype, int64_t M, int64_t N, int64_t K, float slope, int accumulate, void *workspace,

@@ -33,7 +33,7 @@ __device__ __forceinline__ float2 row_sum(float a, float b, int G, float2* red, 
 
 // One group of G threads per row (BLOCK: the workgroup), NV vectors of VE elements per thread.  ODD: the width is no multiple of
 // VE, and the row's last vector is cut off.  The workgroups stay, 16 waves a CU, with weight and bias in their registers (12544 x
-// 4096 bf16: 35 us, 5.9 TB/s; one workgroup per row 43; reading weight and bias again for every row 44).
+// 4096 bf16: 36 us, 5.7 TB/s; one workgroup per row 43; reading weight and bias again for every row 44).
 template <typename T, int NV, bool BLOCK, bool ODD>
 __global__ void __launch_bounds__(BLOCK ? 512 : 256) ln_fwd_kernel(const T* __restrict__ x, long long xs, const float* __restrict__ w,
                                                                    const float* __restrict__ b, T* __restrict__ y,
@@ -282,7 +282,7 @@ __device__ __forceinline__ void column_sums(const BwdArgs& g, int block, float* 
 }
 
 // dx by rows as in the forward pass.  ACC: the thread that holds a column of dx sums its dw and db too, over the rows that its
-// workgroup meets: x and dy are read once for all three (200704 x 256 bf16: 55 us, 5.6 TB/s; 53 + 114 as two kernels).  That needs
+// workgroup meets: x and dy are read once for all three (200704 x 256 bf16: 60 us, 5.1 TB/s; 53 + 114 as two kernels).  That needs
 // many rows per workgroup, or the partial sums outgrow them; for few rows the column sums are other workgroups of the same launch.
 // Four waves a SIMD at least, as the plan counts on: odd bf16 rows took 130 registers and then 188 us where 50000 x 1470 takes 130.
 template <typename T, int NV, bool BLOCK, bool ACC, bool ODD>
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256, 4) ln_bwd_kernel(BwdArgs g)
         }
     }
     int slot = 0;
-    for (long long row = first; row < g.rows; row += stride) {   // (with the next row ahead, as in the forward pass, 200704 x 256 bf16 takes 75 us for 55)
+    for (long long row = first; row < g.rows; row += stride) {   // (with the next row ahead, as in the forward pass, 200704 x 256 bf16 takes 75 us for 60)
         const float mu = g.mean[row], r = g.rstd[row];
         float h[NV][VE], d[NV][VE], s1 = 0.0f, s2 = 0.0f;
         T xr[NV][VE], dr[NV][VE];
@@ -381,8 +381,8 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 256, 4) ln_bwd_kernel(BwdArgs g)
 }
 
 // Rows of more than 1024 vectors, up to 4096 (eight of x and of dy per thread do not fit).  ACC: with the sums of dw and db, in workgroups
-// of up to 512 (2000 x 16384 bf16: 63 us, with column sums by other workgroups 80).  fp32 rows fit five waves a SIMD: 2500 x 9000
-// 92 us against 131 with four.
+// of up to 512 (2000 x 16384 bf16: 56 us, with column sums by other workgroups 80).  fp32 rows fit five waves a SIMD: 2500 x 9000
+// 84 us against 131 with four.
 template <typename T, int NV, bool ACC, bool ODD>
 __global__ void __launch_bounds__(ACC ? 512 : 1024, ACC ? 1 : (sizeof(T) == 4 ? 5 : 4)) ln_bwd_wide_kernel(BwdArgs g) {
     constexpr int VE = 16 / sizeof(T);
@@ -536,7 +536,7 @@ struct Shape { int nv, lg, threads; bool wide = false; };
 // 126 in workgroups of 128, 50000 rows backward; without sums three fit: 74 against 85 forward).  Longer rows have two vectors per
 // thread (4096 bf16 columns: 43 us against 49 with one, 12544 rows forward), `block_most` in a workgroup of 512, and the wide kernels'
 // four or eight (`wide_most`) in one of up to 1024 (forward, with four: 3000 x 12000 bf16 45 us against 52 in the wide form, which takes
-// 2500 x 20000 in 72 us where three readings of the row take 135; backward, 104 in the wide form against 139).
+// 2500 x 20000 in 76 us where three readings of the row take 135; backward, 104 in the wide form against 139).
 Shape ln_shape(int cols, int esize, int wave_most, int block_most, int wide_most) {
     const long long vecs = yfs_cdiv(cols, 16 / esize);
     for (int lg = 3; lg <= 6; ++lg)

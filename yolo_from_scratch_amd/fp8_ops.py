@@ -126,8 +126,9 @@ def _bias(b, n, what):
 def fp8_matmul(x, w, bias=None, slope=None, out_dtype=None):
     """y [..., n] = leaky(Q(x) W^T + bias) for x [..., k] (fp32, bf16 or fp16; quantised by rows inside the call) and an
     ``Fp8Tensor`` w [n, k].  ``slope``: of a LeakyReLU behind the product (None: none).  ``out_dtype``: fp32, bf16 or fp16
-    (default: x's).  Sums are fp32 when the output is; towards 16 bits the 8-bit matrix instruction sums a block of 128 with
-    about 16 bits behind its largest product, 1 / 64 of the output's own rounding.  Not differentiable: ``backward()`` through the
+    (default: x's).  Sums are fp32 when the output is; towards 16 bits the 8-bit matrix instruction keeps 16 bits behind the
+    largest product of a block of 128: an output is off by 2^-9 of that product for each block at most (1.5e-5 of the outputs'
+    norm), which outputs whose products cancel can see beside their own rounding.  Not differentiable: ``backward()`` through the
     result raises (``torch.autograd.grad`` for tensors in front of it leaves its part out); for gradients ``fp8_linear``."""
     if not isinstance(w, Fp8Tensor):
         raise L.YfsError(f"fp8_matmul: w must be an Fp8Tensor (quantize_fp8), got {type(w).__name__}")
