@@ -3,6 +3,8 @@ import os
 import subprocess
 import sys
 
+import pytest
+
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "yolo_from_scratch_amd", "csrc")
 
 
@@ -17,3 +19,12 @@ def test_library_needs_no_torch():
     assert "../libyfs.so" in without and "torch_binding.cpp" not in without and "_binding.so" in without
     both = _plan(sys.executable)
     assert "../libyfs.so" in both and "torch_binding.cpp -o ../_binding.so" in both
+
+
+def test_extension_module_refuses_an_older_library(monkeypatch):
+    from types import SimpleNamespace
+    from yolo_from_scratch_amd import _lib as L
+    monkeypatch.setattr(L, "_binding", None)
+    monkeypatch.setattr(L, "_lib", SimpleNamespace(yfs_version=lambda: 300))
+    with pytest.raises(L.YfsError, match="version 300"):
+        L.binding()

@@ -86,6 +86,8 @@ def binding():
         except ImportError as e:
             raise YfsError(f"yolo_from_scratch_amd/_binding.so cannot be loaded ({e}): build it with "
                            f"`make -C {os.path.join(_HERE, 'csrc')}`. There is no CPU fallback.") from e
+        if lib().yfs_version() < 301:      # (dropout's p was a float before)
+            raise YfsError(f"{LIB_PATH} is version {lib().yfs_version()}, _binding.so calls version 301: build both")
         names = ("yfs_last_error", "yfs_layer_norm_fwd", "yfs_layer_norm_bwd", "yfs_layer_norm_bwd_workspace_bytes",
                  "yfs_dropout_fwd", "yfs_dropout_bwd", "yfs_fp8_matmul", "yfs_fp8_matmul_workspace_bytes", "yfs_fp8_linear_saved_bytes",
                  "yfs_fp8_linear_fwd_workspace_bytes", "yfs_fp8_linear_bwd_workspace_bytes", "yfs_fp8_linear_fwd",
